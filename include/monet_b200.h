@@ -5,7 +5,8 @@
  *
  * Conventions
  *   - Every pointer is a DEVICE pointer unless the parameter name ends in
- *     `_host`.  All activations are fp32.  Nothing here allocates device
+ *     `_host`.  All activations are fp32, except where an entry takes a dtype
+ *     (layer norm, dropout).  Nothing here allocates device
  *     memory: outputs and workspaces are supplied by the caller (the Python
  *     operators obtain them from PyTorch's caching allocator so that MONeT's
  *     memory profiler, monet/meminfo.py:231-243, keeps measuring the truth).
@@ -371,6 +372,62 @@ int mb_conv2d_wgrad_smallc(const float* xp, const float* dy, float* dwp, float* 
  * the first pipeline wait that timed out (the kernel then gave up cleanly).
  * Synchronises the device.  reset != 0 clears it.                            */
 int mb_conv_device_status(int reset);
+
+/* ---- layer norm and dropout (replace lrln.cpp, lrln.cu, ln.py and the autograd-backed
+ * dropout of elementary.py:5-95) --------------------------------------------------------- */
+
+/* Element types of the entries below; all arithmetic is fp32, results are rounded once.     */
+enum { MB_F32 = 0, MB_BF16 = 1, MB_F16 = 2 };
+
+/* Dropout whose mask is a function of (seed, offset, element index) and is never stored.
+ * Philox-4x32-10 keyed by the 64-bit seed (*seed, DEVICE memory, so that a captured graph draws
+ * anew when the seed changes) maps the counter (i/8 low, i/8 high, offset, h) to four words,
+ * i.e. eight 16-bit halves, low half first; half i%8 of h = 0 is the upper and that of h = 1 the
+ * lower half of element i's 32-bit number u.  Dropped (exactly 0, whatever it held) when
+ * u < round(p * 2^32), else multiplied by 1/(1-p).  p in [0, 1].  `offset` tells the dropouts of
+ * a network that share a seed apart.                                                        */
+typedef struct {
+  double p;
+  const long long* seed;  /* device, 8-byte aligned; may be NULL when p rounds to 0          */
+  unsigned offset;
+} mb_dropout_desc;
+
+/* y = dropout(x), element index = position in the buffer.  The backward is the same call on the
+ * gradient.  y may alias x.                                                                 */
+int mb_dropout(const void* x, void* y, size_t n, int dtype, const mb_dropout_desc* d, void* stream);
+
+typedef struct {
+  size_t rows, cols;      /* cols = product of the normalised shape, below 2^31              */
+  size_t ld_a, ld_b, ld_c; /* row strides, in elements, of an entry's first, second and third
+                            * activation input; 0 repeats one row.  Outputs are dense.       */
+  int dtype;              /* activations and their gradients                                 */
+  int param_dtype;        /* weight, bias and their gradients: MB_F32 or the activations'    */
+  float eps;
+} mb_ln_desc;
+
+/* v = x, or residual + dropout(x) when `residual` is given (`drop` NULL: nothing dropped; element
+ * index = row * cols + column);  y = (v - mean) * rstd * weight + bias per row, with
+ * rstd = 1/sqrt(biased variance + eps).  `weight` and `bias` may be NULL (one, zero).  Writes
+ * mean[rows], rstd[rows] and, when non-NULL, `sum` = v.  y may alias x or the residual if that is
+ * dense; so may `sum` (not the one that y aliases).  ld_a: x, ld_b: residual.                */
+int mb_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias,
+                      void* y, void* sum, float* mean, float* rstd, const mb_ln_desc* d,
+                      const mb_dropout_desc* drop, void* stream);
+/* Bytes of scratch mb_layer_norm_bwd needs.                                                 */
+size_t mb_layer_norm_workspace_bytes(const mb_ln_desc* d);
+/* Backward of the above.  `kept` is v (kept_is_output = 0: xhat = (v - mean) * rstd) or the output
+ * y (1: xhat = (y - bias) / weight; needs no mean; a weight of zero is undefined, as for batch norm,
+ * and gives NaN).  With g = dy * weight:
+ *   dv = rstd * (g - mean(g) - xhat * mean(g * xhat)) (+ dsum, the gradient of `sum`, if given),
+ *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy  (either may be NULL).
+ * dv goes to `dv`; dropout(dv), the gradient of x, to `dx` when that is non-NULL.  The sums over
+ * rows are added in a fixed order: two calls on the same inputs agree bit for bit.
+ * dv and dx may alias dy, kept or dsum if that is dense.  ld_a: dy, ld_b: kept, ld_c: dsum.  */
+int mb_layer_norm_bwd(const void* dy, const void* kept, int kept_is_output, const void* dsum,
+                      const void* weight, const void* bias, const float* mean, const float* rstd,
+                      void* dv, void* dx, void* dweight, void* dbias, const mb_ln_desc* d,
+                      const mb_dropout_desc* drop, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 /* ---- diagnostics (NOT part of the drop-in boundary: nothing in the operator library calls
  * them; they exist for the bench harness and for kernel work and may change freely) -------- */

@@ -30,6 +30,15 @@ class BnDesc(C.Structure):
                 ("eps", C.c_float), ("momentum", C.c_float)]
 
 
+class DropoutDesc(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_void_p), ("offset", C.c_uint)]
+
+
+class LnDesc(C.Structure):
+    _fields_ = [(n, C.c_size_t) for n in ("rows", "cols", "ld_a", "ld_b", "ld_c")] + [
+        ("dtype", C.c_int), ("param_dtype", C.c_int), ("eps", C.c_float)]
+
+
 class ConvDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in
                 ("N", "C", "H", "W", "K", "R", "S", "P", "Q", "stride_h", "stride_w", "pad_h",
@@ -38,6 +47,7 @@ class ConvDesc(C.Structure):
 
 MB_CONV_FPROP, MB_CONV_DGRAD, MB_CONV_WGRAD = 0, 1, 2
 MB_CAT_MAX_PIECES = 8
+MB_F32, MB_BF16, MB_F16 = 0, 1, 2
 
 
 # name -> (restype, argtypes); every symbol of include/monet_b200.h
@@ -105,6 +115,11 @@ PROTOTYPES = {
     "mb_cat_rows": (C.c_int, [c_f, C.POINTER(C.c_void_p), C.POINTER(C.c_int), C.c_int, c_sz, C.c_int, c_f]),
     "mb_global_avgpool_fwd": (C.c_int, [c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "mb_global_avgpool_bwd": (C.c_int, [c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
+    "mb_dropout": (C.c_int, [c_f, c_f, c_sz, C.c_int, C.POINTER(DropoutDesc), c_f]),
+    "mb_layer_norm_fwd": (C.c_int, [c_f] * 8 + [C.POINTER(LnDesc), C.POINTER(DropoutDesc), c_f]),
+    "mb_layer_norm_workspace_bytes": (c_sz, [C.POINTER(LnDesc)]),
+    "mb_layer_norm_bwd": (C.c_int, [c_f, c_f, C.c_int] + [c_f] * 9 + [C.POINTER(LnDesc), C.POINTER(DropoutDesc),
+                                                                    c_f, c_sz, c_f]),
 }
 
 _lib = None

@@ -10,6 +10,8 @@ the layout flag.  Anything else is first made contiguous.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 
 import torch
 
@@ -980,3 +982,240 @@ def depthwise_bwd(dy, x, w, stride, padding, dilation, groups, need=(True, True,
                                        _stream()), "depthwise_wgrad")
         dw = dwt.t().reshape(d.C, 1, d.R, d.S) if need[1] else None
     return dx, dw, db
+
+
+# ------------------------------------------------------------- dropout and layer norm
+# These take float32, bfloat16 and float16 activations; arithmetic is fp32, results are rounded
+# once.  They run on the device of their first tensor, on that device's current stream.
+
+from ._lib import DropoutDesc, LnDesc  # noqa: E402
+
+_DTYPE_CODE = {torch.float32: _lib.MB_F32, torch.bfloat16: _lib.MB_BF16, torch.float16: _lib.MB_F16}
+
+
+def _on_its_device(fn):
+    """Runs `fn` with the device of its first tensor as the current one."""
+    @functools.wraps(fn)
+    def call(t, *args, **kwargs):
+        if t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                return fn(t, *args, **kwargs)
+        return fn(t, *args, **kwargs)
+    return call
+
+
+def _act_dtype(first: torch.Tensor, **others) -> int:
+    """The dtype code of `first`; every other (non-None) activation must match it in type and device."""
+    if not first.is_cuda:
+        raise RuntimeError("monet_b200 operators run on CUDA tensors only (no CPU fallback)")
+    code = _DTYPE_CODE.get(first.dtype)
+    if code is None:
+        raise RuntimeError(f"monet_b200: unsupported dtype {first.dtype} (float32, bfloat16, float16)")
+    for name, t in others.items():
+        if t is None:
+            continue
+        if t.dtype != first.dtype or t.device != first.device:
+            raise RuntimeError(f"monet_b200: {name} must be {first.dtype} on {first.device}, got {t.dtype} on {t.device}")
+    return code
+
+
+def dropout_seed(device) -> torch.Tensor:
+    """A 64-bit dropout seed drawn from PyTorch's generator of `device` (so ``torch.manual_seed``
+    governs it, and a captured graph draws a new one at every replay)."""
+    return torch.randint(-2 ** 62, 2 ** 62, (1,), dtype=torch.int64, device=device)
+
+
+def _drop_desc(x: torch.Tensor, p: float, seed, offset: int):
+    """(descriptor or None when nothing is dropped); checks the seed."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"monet_b200: dropout probability must lie in [0, 1], got {p}")
+    if p * 2.0 ** 32 < 0.5:
+        return None
+    if not (torch.is_tensor(seed) and seed.dtype == torch.int64 and seed.numel() == 1 and seed.device == x.device):
+        raise RuntimeError(f"monet_b200: the dropout seed must be an int64 tensor of one element on {x.device}")
+    if not 0 <= int(offset) < 2 ** 32:
+        raise RuntimeError(f"monet_b200: dropout offset must lie in [0, 2^32), got {offset}")
+    return DropoutDesc(p, seed.data_ptr(), int(offset))
+
+
+@_on_its_device
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool = False) -> torch.Tensor:
+    """x / (1 - p) where kept, 0 where dropped.  Which elements are dropped depends on `seed` (an
+    int64 tensor of one element on x's device, ``dropout_seed``), `offset` (tells dropouts that
+    share a seed apart) and the element's position in physical order, so the mask is not stored:
+    ``dropout_bwd`` and a repeated forward draw the same one.  The generator is specified at
+    ``mb_dropout`` in the header."""
+    code = _act_dtype(x)
+    desc = _drop_desc(x, p, seed, offset) or DropoutDesc(0.0, None, 0)
+    xd = dense(x)
+    y = xd if (inplace and xd is x) else torch.empty_like(xd)
+    check(lib().mb_dropout(xd.data_ptr(), y.data_ptr(), xd.numel(), code, C.byref(desc), _stream()), "dropout")
+    return y
+
+
+def dropout_bwd(dy: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool = False) -> torch.Tensor:
+    """The gradient of ``dropout`` for the same p, seed and offset; `dy` in the physical order of
+    the forward's tensor."""
+    return dropout(dy, p, seed, offset, inplace)
+
+
+def _norm_geometry(x: torch.Tensor, normalized_shape):
+    """(rows, cols) of x seen as rows of the trailing dimensions `normalized_shape`."""
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(s) for s in normalized_shape)
+    if not shape or x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
+        raise RuntimeError(f"monet_b200: normalized_shape {shape} is not the end of the input's shape {tuple(x.shape)}")
+    cols = math.prod(shape)
+    if cols == 0:
+        raise RuntimeError("monet_b200: layer norm over zero values")
+    return x.numel() // cols, cols
+
+
+def _as_rows(t: torch.Tensor, rows: int, cols: int):
+    """(tensor, row stride): `t` itself when its rows are dense and evenly spaced, else a copy."""
+    if t.is_contiguous():
+        return t, cols
+    try:
+        v = t.view(rows, cols)
+    except RuntimeError:
+        return t.contiguous(), cols
+    if cols > 1 and v.stride(1) != 1:
+        return t.contiguous(), cols
+    return v, v.stride(0) if rows > 1 else cols
+
+
+def _norm_params(x: torch.Tensor, cols: int, code: int, weight, bias):
+    """(weight, bias, dtype code) made dense; they are fp32 or of x's type, and alike."""
+    kind = None
+    out = []
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            if t.device != x.device or t.numel() != cols:
+                raise RuntimeError(f"monet_b200: {name} must have {cols} values on {x.device}")
+            if t.dtype not in (torch.float32, x.dtype) or (kind is not None and t.dtype != kind):
+                raise RuntimeError(f"monet_b200: weight and bias must both be float32 or both {x.dtype}, got {name} {t.dtype}")
+            kind = t.dtype
+            t = t.detach()
+            t = t if t.is_contiguous() else t.contiguous()
+        out.append(t)
+    return out[0], out[1], _lib.MB_F32 if kind in (None, torch.float32) else code
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stat(t: torch.Tensor, x: torch.Tensor, rows: int, name: str) -> torch.Tensor:
+    if t.dtype != torch.float32 or t.device != x.device or t.numel() != rows:
+        raise RuntimeError(f"monet_b200: {name} must hold {rows} float32 values on {x.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, drop, want_sum, inplace):
+    code = _act_dtype(x, residual=residual)
+    rows, cols = _norm_geometry(x, normalized_shape)
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError("monet_b200: residual and input shapes differ (broadcasting is not supported)")
+    w, b, pcode = _norm_params(x, cols, code, weight, bias)
+    xr, lda = _as_rows(x, rows, cols)
+    rr, ldb = _as_rows(residual, rows, cols) if residual is not None else (None, 0)
+    y = x if inplace and x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_sum else None
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    mean, rstd = stats.unbind(0)
+    d = LnDesc(rows, cols, lda, ldb, 0, code, pcode, float(eps))
+    check(lib().mb_layer_norm_fwd(xr.data_ptr(), _ptr(rr), _ptr(w), _ptr(b), y.data_ptr(), _ptr(z),
+                                  mean.data_ptr(), rstd.data_ptr(), C.byref(d),
+                                  C.byref(drop) if drop is not None else None, _stream()), "layer_norm_fwd")
+    return y, z, mean, rstd
+
+
+def _layer_norm_bwd(dy, kept, from_output, dz, normalized_shape, weight, bias, mean, rstd, drop,
+                    need_weight, need_bias):
+    code = _act_dtype(dy, kept=kept, dz=dz)
+    rows, cols = _norm_geometry(kept, normalized_shape)
+    if dy.shape != kept.shape or (dz is not None and dz.shape != kept.shape):
+        raise RuntimeError("monet_b200: gradient and activation shapes differ")
+    w, b, pcode = _norm_params(kept, cols, code, weight, bias)
+    rstd = _row_stat(rstd, dy, rows, "rstd")
+    mean = _row_stat(mean, dy, rows, "mean") if mean is not None else None
+    gr, lda = _as_rows(dy, rows, cols)
+    kr, ldb = _as_rows(kept, rows, cols)
+    zr, ldc = _as_rows(dz, rows, cols) if dz is not None else (None, 0)
+    device = dy.device
+    dv = torch.empty(dy.shape, dtype=dy.dtype, device=device)
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=device) if drop is not None else None
+    pdtype = torch.float32 if pcode == _lib.MB_F32 else dy.dtype
+    pshape = tuple(kept.shape[kept.dim() - (1 if isinstance(normalized_shape, int) else len(normalized_shape)):])
+    dw = torch.empty(pshape, dtype=pdtype, device=device) if need_weight else None
+    db = torch.empty(pshape, dtype=pdtype, device=device) if need_bias else None
+    d = LnDesc(rows, cols, lda, ldb, ldc, code, pcode, 0.0)
+    nbytes = lib().mb_layer_norm_workspace_bytes(C.byref(d)) if need_weight or need_bias else 0
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    check(lib().mb_layer_norm_bwd(gr.data_ptr(), kr.data_ptr(), int(from_output), _ptr(zr), _ptr(w), _ptr(b),
+                                  _ptr(mean), rstd.data_ptr(), dv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
+                                  C.byref(d), C.byref(drop) if drop is not None else None,
+                                  ws.data_ptr(), ws.numel(), _stream()), "layer_norm_bwd")
+    return dv, dx, dw, db
+
+
+@_on_its_device
+def layer_norm(x: torch.Tensor, normalized_shape, weight=None, bias=None, eps: float = 1e-5, inplace: bool = False):
+    """(y, mean, rstd): layer norm over the trailing dimensions `normalized_shape`; mean and rstd
+    (= 1/sqrt(biased variance + eps)) are fp32, one value a row.  `weight` and `bias` are fp32 or of
+    x's type.  `inplace` overwrites a contiguous x."""
+    y, _, mean, rstd = _layer_norm_fwd(x, None, normalized_shape, weight, bias, eps, None, False, inplace)
+    return y, mean, rstd
+
+
+@_on_its_device
+def layer_norm_bwd_from_input(dy, x, normalized_shape, weight, mean, rstd, need_weight: bool = True, need_bias: bool = True):
+    """(dx, dweight, dbias) from the stored INPUT; the parameters' gradients have the weight's type
+    (fp32 without one) and are None when not needed."""
+    dx, _, dw, db = _layer_norm_bwd(dy, x, False, None, normalized_shape, weight, None, mean, rstd, None,
+                                    need_weight, need_bias)
+    return dx, dw, db
+
+
+@_on_its_device
+def layer_norm_bwd_from_output(dy, y, normalized_shape, weight, bias, rstd, need_weight: bool = True, need_bias: bool = True):
+    """(dx, dweight, dbias) from the stored OUTPUT, xhat = (y - bias) / weight: the input need not
+    be kept and the forward can run in place.  A weight of zero is undefined (NaN), as for batch norm,
+    and y's rounding enters xhat divided by the weight."""
+    dx, _, dw, db = _layer_norm_bwd(dy, y, True, None, normalized_shape, weight, bias, None, rstd, None,
+                                    need_weight, need_bias)
+    return dx, dw, db
+
+
+@_on_its_device
+def dropout_add_layer_norm(x, residual, normalized_shape, weight=None, bias=None, eps: float = 1e-5, p: float = 0.0,
+                           seed=None, offset: int = 0, want_sum: bool = True, inplace: bool = False):
+    """(y, z, mean, rstd) with z = residual + dropout(x) and y = layer_norm(z), in one pass.  The
+    dropout is ``dropout``'s with the element's row-major index; z is None unless `want_sum` (a
+    pre-norm network carries it on; its statistics are those of the unrounded sum)."""
+    drop = _drop_desc(x, p, seed, offset)
+    return _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, drop, want_sum, inplace)
+
+
+def _pair_of_gradients(dv, dx, dw, db):
+    # without dropout both operands of the sum have the same gradient: shared, not copied
+    return (dv if dx is None else dx), dv, dw, db
+
+
+@_on_its_device
+def dropout_add_layer_norm_bwd_from_sum(dy, z, normalized_shape, weight, mean, rstd, p: float = 0.0, seed=None,
+                                        offset: int = 0, dz=None, need_weight: bool = True, need_bias: bool = True):
+    """(dx, dresidual, dweight, dbias) from the stored SUM z; `dz` is the gradient that z receives
+    from elsewhere.  dx is dresidual itself when nothing is dropped."""
+    drop = _drop_desc(dy, p, seed, offset)
+    return _pair_of_gradients(*_layer_norm_bwd(dy, z, False, dz, normalized_shape, weight, None, mean, rstd, drop,
+                                               need_weight, need_bias))
+
+
+@_on_its_device
+def dropout_add_layer_norm_bwd_from_output(dy, y, normalized_shape, weight, bias, rstd, p: float = 0.0, seed=None,
+                                           offset: int = 0, dz=None, need_weight: bool = True, need_bias: bool = True):
+    """The same from the stored OUTPUT y, xhat = (y - bias) / weight (``layer_norm_bwd_from_output``)."""
+    drop = _drop_desc(dy, p, seed, offset)
+    return _pair_of_gradients(*_layer_norm_bwd(dy, y, True, dz, normalized_shape, weight, bias, None, rstd, drop,
+                                               need_weight, need_bias))

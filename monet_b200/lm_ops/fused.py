@@ -1,4 +1,5 @@
-"""Fused operators: batch norm + ReLU, batch norm + residual add + ReLU, add + ReLU.
+"""Fused operators: batch norm + ReLU, batch norm + residual add + ReLU, add + ReLU, and
+dropout + residual add + layer norm.
 
 The reference has no such operators: its graph runs ``aten::batch_norm``, ``aten::add`` and
 ``aten::relu`` as separate nodes (monet/lm_ops/bn.py, funcs.py, relu.py), each a full pass
@@ -10,14 +11,18 @@ names of their own, ``monet::batch_norm_relu`` (and ``_relu6``),
 rewriter (``runner.fuse_graph``) produces those nodes from the unfused pattern.
 
 Argument order = the batch-norm node's arguments, then the residual:
-``(x, weight, bias, running_mean, running_var, training, momentum, eps, cudnn, residual)``.
+``(x, weight, bias, running_mean, running_var, training, momentum, eps, cudnn, residual)``;
+``monet::dropout_add_layer_norm`` takes
+``(x, residual, normalized_shape, weight, bias, eps, p, training)``.
 """
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from .. import functional as F
-from .base import COMMON_MODES, OP, InputStorage, OutputStorage, implements
+from .base import COMMON_MODES, OP, InputStorage, IntermediateStorage, OutputStorage, implements
+from .dropout import training_p
 
 
 class _FusedBatchNorm(OP):
@@ -144,3 +149,66 @@ class AddReLU(OP):
                 del stored[0]
             alpha = self.params if self.params is not None else 1.0
             return d, (d if alpha == 1.0 else F.scale(d, alpha))
+
+
+class _DropoutAddLayerNorm(OP):
+    """y = layer_norm(residual + dropout(x)) (the end of a post-norm transformer block) in one pass.
+    The dropout keeps a seed only; ``params`` is (shape, p, seed, mean, rstd)."""
+    params = None
+    inplace = False
+    keeps_sum = False
+
+    def _forward(self, x, residual, normalized_shape, weight, bias, eps, p, training):
+        with torch.no_grad():
+            if self.params is None:
+                p = training_p(p, training)
+                seed = F.dropout_seed(x.device) if p > 0 else None
+            else:
+                p, seed = self.params[1], self.params[2]
+            y, z, mean, rstd = F.dropout_add_layer_norm(
+                x, residual, normalized_shape, weight, bias, eps, p, seed, want_sum=self.keeps_sum,
+                inplace=self.inplace)
+            self.params = list(normalized_shape), p, seed, mean, rstd
+            return y, z
+
+
+@implements(['monet::dropout_add_layer_norm'], COMMON_MODES)
+class SumActDropoutAddLayerNorm(_DropoutAddLayerNorm):
+    """Keeps the sum residual + dropout(x) beside the output."""
+    backward_storage = [InputStorage(3, 4), IntermediateStorage(lambda shape: 4 * np.prod(shape))]
+    keeps_sum = True
+
+    def forward(self, x, residual, normalized_shape, weight=None, bias=None, eps=1e-5, p=0.0, training=True):
+        return self._forward(x, residual, normalized_shape, weight, bias, eps, p, training)
+
+    def backward(self, grad_output, stored, nodel=False):
+        with torch.no_grad():
+            weight, bias, z = stored
+            shape, p, seed, mean, rstd = self.params
+            grads = F.dropout_add_layer_norm_bwd_from_sum(
+                grad_output, z, shape, weight, mean, rstd, p, seed, need_weight=weight is not None,
+                need_bias=bias is not None)
+            if not nodel:
+                del stored[2], stored[1], stored[0]
+            return tuple(g for g in grads if g is not None)
+
+
+@implements(['monet::dropout_add_layer_norm'], ['multiway', 'multiway_newnode', 'conv_multiway_newnode'])
+class OutputActDropoutAddLayerNorm(_DropoutAddLayerNorm):
+    """Keeps nothing but the output (which the next operator reads anyway): neither x nor the sum.
+    Every weight must be non-zero (ln.OutputActLayerNorm)."""
+    backward_storage = [InputStorage(3, 4), OutputStorage()]
+
+    def forward(self, x, residual, normalized_shape, weight=None, bias=None, eps=1e-5, p=0.0, training=True):
+        return self._forward(x, residual, normalized_shape, weight, bias, eps, p, training)[0]
+
+    def backward(self, grad_output, stored, nodel=False):
+        with torch.no_grad():
+            weight, bias, y = stored
+            shape, p, seed, _, rstd = self.params
+            grads = F.dropout_add_layer_norm_bwd_from_output(
+                grad_output, y, shape, weight, bias, rstd, p, seed, need_weight=weight is not None,
+                need_bias=bias is not None)
+            if not nodel:
+                del stored[2], stored[1], stored[0]
+            return tuple(g for g in grads if g is not None)

@@ -63,7 +63,8 @@ def _as_list(v, n=2):
 
 def extract_graph(model: nn.Module) -> Tuple[List[Node], int]:
     """(nodes, id of the output node) for a model made of conv / batch-norm / ReLU / ReLU6 /
-    max-pool / adaptive-avg-pool / linear / dropout modules joined by add, flatten and cat."""
+    max-pool / adaptive-avg-pool / linear / dropout / layer-norm modules joined by add, flatten and
+    cat."""
     gm = torch.fx.symbolic_trace(model)
     mods = dict(gm.named_modules())
     nodes: List[Node] = []
@@ -130,6 +131,11 @@ def extract_graph(model: nn.Module) -> Tuple[List[Node], int]:
                      fn.target)
             elif isinstance(m, nn.Dropout):
                 emit(fn, 'aten::dropout', [x, Arg('const', m.p), Arg('const', True)], fn.target)
+            elif isinstance(m, nn.LayerNorm):
+                affine = lambda name: P(name) if getattr(m, name) is not None else Arg('const', None)  # noqa: E731
+                emit(fn, 'aten::layer_norm',
+                     [x, Arg('const', list(m.normalized_shape)), affine('weight'), affine('bias'),
+                      Arg('const', m.eps), Arg('const', True)], fn.target)
             else:
                 raise NotImplementedError(f"module {type(m).__name__} at {fn.target}")
         elif fn.op == 'call_function':
@@ -163,7 +169,9 @@ def fuse_graph(nodes: List[Node], out_id: int) -> Tuple[List[Node], int]:
     * ``batch_norm -> add(., r) -> relu``    => ``monet::batch_norm_add_relu`` with ``r`` appended
       to the batch-norm arguments, placed where the add was (``r`` may be produced after the
       batch norm, e.g. by a downsample branch);
-    * ``add -> relu`` (any other add)        => ``monet::add_relu``.
+    * ``add -> relu`` (any other add)        => ``monet::add_relu``;
+    * ``dropout -> add(., r) -> layer_norm`` => ``monet::dropout_add_layer_norm`` (also without the
+      dropout), placed where the layer norm was.
 
     A link is fused only when the intermediate value has no other reader, the batch norm is
     in training mode and the add has alpha == 1 and two distinct node operands."""
@@ -214,6 +222,17 @@ def fuse_graph(nodes: List[Node], out_id: int) -> Tuple[List[Node], int]:
             n.op = 'monet::add_relu'
             removed.add(r.id)
             alias[r.id] = n.id
+        elif r is not None and r.op == 'aten::layer_norm':
+            x, residual, p = n.args[0], n.args[1], 0.0
+            for a, b in ((n.args[0], n.args[1]), (n.args[1], n.args[0])):
+                d = by_id[a.value]
+                if d.op == 'aten::dropout' and sole_user(d) is n and d.args[2].value:
+                    x, residual, p = d.args[0], b, float(d.args[1].value)
+                    removed.add(d.id)
+                    break
+            r.op = 'monet::dropout_add_layer_norm'
+            r.args = [x, residual] + r.args[1:5] + [Arg('const', p), Arg('const', True)]
+            removed.add(n.id)
 
     kept = [n for n in nodes if n.id not in removed]
     renumber = {n.id: i for i, n in enumerate(kept)}
@@ -274,12 +293,21 @@ def store_all(nodes: List[Node], n: Node) -> Choice:
     return Choice()
 
 
+# Producers whose output no backward of their own reads and that return memory of their own: a sole
+# reader may overwrite it.
+_NEVER_READ_AGAIN = ('aten::addmm', 'aten::_convolution', 'aten::add')
+
+
 def low_memory(nodes: List[Node], n: Node) -> Choice:
-    """In-place batch norm that backpropagates from its output, ReLU kept as nothing at all
+    """In-place batch norm and layer norm that backpropagate from their output, ReLU kept as nothing at all
     (recomputed from the batch-norm output it reads, gated in backward by that same tensor),
     residual add in place, max-pool keeping 4-bit indices."""
     if n.op == 'aten::batch_norm':
         return Choice(impl=1, inplace=_sole_user(nodes, n))
+    if n.op in ('aten::layer_norm', 'monet::dropout_add_layer_norm'):
+        return Choice(impl=1, inplace=_sole_user(nodes, n) and nodes[n.args[0].value].op in _NEVER_READ_AGAIN)
+    if n.op == 'monet::dropout':
+        return Choice(recompute=True)      # keeps its seed; the same mask is drawn again
     if n.op in ('aten::relu', 'aten::relu_'):
         return Choice(impl=0, inplace=False, recompute=True)
     if n.op in ('aten::hardtanh', 'aten::hardtanh_'):
@@ -321,7 +349,10 @@ class Runner:
 
     def __init__(self, model: nn.Module, policy: Policy = store_all,
                  mode: str = "conv_multiway_newnode", input_requires_grad: bool = False,
-                 fuse: bool = False, channel_sums: bool = True):
+                 fuse: bool = False, channel_sums: bool = True, counter_dropout: bool = False):
+        """``fuse`` rewrites the graph (``fuse_graph``); ``counter_dropout`` runs every dropout that
+        is not part of a fused node as ``monet::dropout``, which stores no mask and can be
+        recomputed."""
         self.model = model
         self.nodes, self.out_id = extract_graph(model)
         if fuse:
@@ -330,6 +361,10 @@ class Runner:
             if not channel_sums:       # batch norms make their own statistics pass
                 for n in self.nodes:
                     n.sums_from = -1
+        if counter_dropout:
+            for n in self.nodes:
+                if n.op == 'aten::dropout':
+                    n.op = 'monet::dropout'
         self.mode = mode
         self.input_requires_grad = input_requires_grad
         self.choices = [policy(self.nodes, n) for n in self.nodes]

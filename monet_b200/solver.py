@@ -80,11 +80,13 @@ def estimate_costs(si, graph, hbm_gbs: float = 6400.0, tensor_tflops: float = 40
     # bytes per output element: (forward, backward) per implementation
     fwd_b = {"aten::batch_norm": 12, "aten::relu": 8, "aten::relu_": 8, "aten::hardtanh": 8,
              "aten::hardtanh_": 8, "aten::add": 12, "aten::add_": 12, "aten::max_pool2d": 20,
-             "aten::cat": 8, "aten::adaptive_avg_pool2d": 8, "aten::dropout": 12}
+             "aten::cat": 8, "aten::adaptive_avg_pool2d": 8, "aten::dropout": 12,
+             "aten::layer_norm": 8, "monet::dropout": 8, "monet::dropout_add_layer_norm": 12}
     bwd_b = {"aten::batch_norm": [20, 20], "aten::relu": [12, 12, 8.2], "aten::relu_": [12, 12, 8.2],
              "aten::hardtanh": [12, 12], "aten::hardtanh_": [12, 12], "aten::add": [0.1], "aten::add_": [0.1],
              "aten::max_pool2d": [40, 20], "aten::cat": [8], "aten::adaptive_avg_pool2d": [8],
-             "aten::dropout": [12]}
+             "aten::dropout": [12], "aten::layer_norm": [12, 12], "monet::dropout": [8],
+             "monet::dropout_add_layer_norm": [16, 16]}
 
     for i in si.nodes:
         for name in ("workspace_mem", "workspace_compute", "recompute_workspace_mem",

@@ -317,3 +317,57 @@ def stem_reference(seed=0, N=4, H=224, W=224):
                 relu=r.detach(), y=y.detach(), dx=xr.grad, dw=wr.grad, dgamma=gr.grad,
                 dbeta=br.grad, mask=relu_mask_bytes(b.detach()), local_idx=local,
                 nibbles=maxpool_nibbles(local))
+
+
+# ------------------------------------------------- layer norm and counter-based dropout, 64 bits
+
+def dropout_numbers(seed: int, offset: int, n: int) -> np.ndarray:
+    """The 32-bit number of each of n elements, as uint32: Philox-4x32-10 (Salmon et al., SC 2011)
+    on the counters (i // 8, offset, half), in numpy's 64-bit unsigned arithmetic."""
+    key = seed % (1 << 64)
+    block = np.arange((n + 7) // 8, dtype=np.uint64)
+    out = []
+    for half in (0, 1):
+        words = philox_words([block & _U32, block >> np.uint64(32), np.uint64(offset), np.uint64(half)], key)
+        out.append(words.view("<u2").reshape(-1)[:n].astype(np.uint32))
+    return (out[0] << np.uint32(16)) | out[1]
+
+
+_U32 = np.uint64(0xFFFFFFFF)
+
+
+def philox_words(counter, key: int) -> np.ndarray:
+    """The four output words of each counter, [blocks, 4] little-endian uint32."""
+    c = [np.atleast_1d(np.asarray(v, dtype=np.uint64)) for v in counter]
+    for r in range(10):
+        k0 = np.uint64(((key & 0xFFFFFFFF) + r * 0x9E3779B9) % (1 << 32))
+        k1 = np.uint64(((key >> 32) + r * 0xBB67AE85) % (1 << 32))
+        a, b = np.uint64(0xD2511F53) * c[0], np.uint64(0xCD9E8D57) * c[2]
+        c = [(b >> np.uint64(32)) ^ c[1] ^ k0, b & _U32, (a >> np.uint64(32)) ^ c[3] ^ k1, a & _U32]
+    words = np.empty((max(v.size for v in c), 4), dtype="<u4")
+    for j in range(4):
+        words[:, j] = c[j]
+    return words
+
+
+def dropout_keep(seed: int, offset: int, n: int, p: float) -> torch.Tensor:
+    """True where an element is kept."""
+    return torch.from_numpy(dropout_numbers(seed, offset, n).astype(np.uint64) >= np.uint64(int(p * 2.0 ** 32 + 0.5)))
+
+
+def layer_norm_forward(v: torch.Tensor, w=None, b=None, eps: float = 1e-5):
+    """(y, mean, rstd) of the rows of a 2-D tensor, in 64 bits."""
+    v = v.double()
+    mean = v.mean(1)
+    rstd = ((v - mean[:, None]) ** 2).mean(1).add(eps).rsqrt()
+    y = (v - mean[:, None]) * rstd[:, None]
+    y = y * w.double() if w is not None else y
+    return (y + b.double() if b is not None else y), mean, rstd
+
+
+def layer_norm_backward(dy: torch.Tensor, xhat: torch.Tensor, w, rstd: torch.Tensor):
+    """(dv, dw, db) for rows normalised to xhat, in 64 bits."""
+    dy, xhat = dy.double(), xhat.double()
+    g = dy * w.double() if w is not None else dy
+    dv = rstd.double()[:, None] * (g - g.mean(1, True) - xhat * (g * xhat).mean(1, True))
+    return dv, (dy * xhat).sum(0), dy.sum(0)
