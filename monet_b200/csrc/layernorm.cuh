@@ -53,7 +53,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-// A row stays in registers when it fits kMaxThreads * K granules per CTA and eight CTAs, K being at
+// A row stays in registers when it fits kMaxTeam * K granules per CTA and eight CTAs, K being at
 // most 4 (8 in a cluster) forward and 2 backward, where each value also has two column sums and a
 // weight; longer rows, and tensors whose rows do not lie on granule boundaries in the same way, take
 // the element-wise kernels.
@@ -61,16 +61,17 @@ constexpr int kRingLimit = 216 * 1024;
 
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-inline bool plan_rows(size_t cols, int elem, int ops, bool backward, int threads, RowPlan* q) {
+inline bool plan_rows(size_t rows, size_t cols, int elem, int ops, bool backward, bool from_y, RowPlan* q) {
+  if (rows >> 30) return false;                              // row numbers are 32-bit, and some steps ahead
   int g = 8;
   while (cols % g) g /= 2;                                   // gcd(cols, 8)
   q->period = 8 / g;
   const size_t most = (cols + (8 - g) + 7) / 8;              // granules a row can touch
   const int k_max = backward ? 2 : 4, k_cluster = backward ? 2 : 8;
-  if (most > static_cast<size_t>(kMaxThreads) * 8 * k_cluster) return false;
+  if (most > static_cast<size_t>(kMaxTeam) * 8 * k_cluster) return false;
   for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
     q->chunk = ceil_div(static_cast<long long>(most), q->cluster);
-    if (q->chunk > kMaxThreads * (q->cluster == 8 ? k_cluster : k_max)) continue;
+    if (q->chunk > kMaxTeam * (q->cluster == 8 ? k_cluster : k_max)) continue;
     if (q->chunk <= 32) {
       q->team = 1;
       while (q->team < q->chunk) q->team *= 2;
@@ -79,19 +80,27 @@ inline bool plan_rows(size_t cols, int elem, int ops, bool backward, int threads
       const int wish = backward ? 256 : 128;
       int k = 1;
       while (k < k_max && ceil_div(q->chunk, 32 * k) * 32 > wish) k *= 2;
-      while (ceil_div(q->chunk, 32 * k) * 32 > kMaxThreads) k *= 2;
+      while (ceil_div(q->chunk, 32 * k) * 32 > kMaxTeam) k *= 2;
       q->per_thread = k;
       q->team = ceil_div(q->chunk, 32 * k) * 32;
     }
+    const int threads = !backward ? 256 : q->per_thread == 1 ? 512 : 768;
     q->groups = q->cluster > 1 || q->team >= threads ? 1 : threads / q->team;
     if (q->team > 32 && q->groups > 15) q->groups = 15;      // named barriers
     const size_t stage = static_cast<size_t>(q->groups) * q->chunk * 8 * elem * ops;
-    const int deep = static_cast<int>((backward ? 200 * 1024 : 64 * 1024) / stage);
-    q->stages = deep > 6 ? 6 : deep < 2 ? 2 : deep;
-    q->smem = stage * q->stages;
-    if (backward && q->groups > 1) {                         // the teams' column sums are folded there
-      const size_t fold = static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * 16 * sizeof(float);
-      if (fold > q->smem) q->smem = fold;
+    if (backward) {
+      // two CTAs per SM of one granule a thread; fp32 weight (and its inverse and the bias) beside the ring
+      const size_t params = static_cast<size_t>(q->chunk) * 32 * (from_y ? 3 : 1);
+      const size_t budget = (q->per_thread == 1 ? 104 : 208) * 1024;
+      const int deep = budget > params ? static_cast<int>((budget - params) / stage) : 0;
+      q->stages = deep > 8 ? 8 : deep < kRows ? kRows : deep;
+      q->smem = stage * q->stages + params;
+      const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * 16 * sizeof(float) : 0;
+      if (fold > q->smem) q->smem = fold;                    // the teams' column sums are folded there
+    } else {
+      const int deep = static_cast<int>(64 * 1024 / stage);
+      q->stages = deep > 6 ? 6 : deep < 2 ? 2 : deep;
+      q->smem = stage * q->stages;
     }
     if (q->smem <= kRingLimit) return true;
   }

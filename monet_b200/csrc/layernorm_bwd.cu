@@ -4,9 +4,15 @@
 namespace mb {
 namespace {
 
-// Backward.  partial[blockIdx.x][0][col] = sum of dy xhat, [1][col] = sum of dy over this CTA's rows.
-template <typename T, int K, bool FROM_Y, bool DSUM, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
+// Backward.  partial[team CTA][0][col] = sum of dy xhat, [1][col] = sum of dy over the CTA's rows.
+//
+// kRows rows are handled between two barriers: their sums (mean(g), mean(g xhat)) are formed from a
+// first reading of the ring, then the rows are read a second time to form dv.  Reading twice costs
+// shared-memory loads but no registers, which the column sums need; the parameters lie in shared
+// memory for the same reason.  With 64 registers a thread two CTAs share an SM, and one computes
+// while the other waits for its barrier.
+template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
+__global__ void __launch_bounds__(K == 1 ? kMaxTeam : kMaxThreads, K == 1 ? 2 : 1) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
   __shared__ WarpSums red;
@@ -14,197 +20,220 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
   constexpr int kOps = DSUM ? 3 : 2;
   const RowWalk at(q, static_cast<int>(p.cols));
   const int granules = EDGE ? static_cast<int>((at.m + p.cols + 7) >> 3) : static_cast<int>(p.cols >> 3);
-  const size_t total = p.rows * p.cols;
   const float inv_n = 1.f / static_cast<float>(p.cols);
-  const unsigned long long key = p.drop.on ? __ldg(p.drop.seed) : 0;
+  const int j0 = at.rank * q.chunk + at.t;           // the thread's granules: j0 + k * team
+  const int rows = static_cast<int>(p.rows), step = static_cast<int>(at.step);
 
-  long long col[K];
   uint32_t mask[K];
-  float w[K][8], iw[FROM_Y ? K : 1][8], b[FROM_Y ? K : 1][8];
-  float aw[K][8], ab[K][8];
+  float2 aw[K][4], ab[K][4];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int jl = at.t + k * q.team, j = at.rank * q.chunk + jl;
-    col[k] = static_cast<long long>(j) * 8 - at.m;
-    mask[k] = jl < q.chunk && j < granules ? 0xffu : 0u;
-    if (EDGE && mask[k]) {
-      if (col[k] < 0) mask[k] &= 0xffu << -col[k];
-      if (col[k] + 8 > static_cast<long long>(p.cols)) mask[k] &= 0xffu >> (col[k] + 8 - static_cast<long long>(p.cols));
-    }
-    param8<T>(p.w, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 1.f, w[k]);
-    if (FROM_Y) {
-      param8<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 0.f, b[FROM_Y ? k : 0]);
+    mask[k] = column_mask<EDGE>(at, q, granules, static_cast<int>(p.cols), k);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) iw[FROM_Y ? k : 0][i] = 1.f / w[k][i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) aw[k][i] = ab[k][i] = 0.f;
+    for (int i = 0; i < 4; ++i) aw[k][i] = ab[k][i] = make_float2(0.f, 0.f);
   }
 
   const int plane = q.chunk;
   const int per_op = plane * kPlanes<T>, per_stage = per_op * kOps;
-  uint4* mine = ring + static_cast<size_t>(at.group) * q.stages * per_stage + at.t;
-  const uint32_t mine_u = sm100::smem_u32(mine);
-  const T* const src[3] = {static_cast<const T*>(p.a), static_cast<const T*>(p.b), static_cast<const T*>(p.c)};
-  const size_t ld[3] = {p.ld_a, p.ld_b, p.ld_c};
+  uint4* mine = ring + at.group * q.stages * per_stage + at.t;
+  float4* const ws = reinterpret_cast<float4*>(ring) + q.stages * q.groups * per_stage + at.t;
 
-  auto fetch = [&](size_t row, int stage) {
-    if (row < p.rows) {
+  auto fetch = [&](int row, int stage) {
+    if (row < rows) {
+      const uint32_t dst = sm100::smem_u32(mine) + stage * per_stage * 16;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!mask[k]) continue;
-        const int j = at.rank * q.chunk + at.t + k * q.team;
-        const uint32_t dst = mine_u + (stage * per_stage + k * q.team) * 16;
-#pragma unroll
-        for (int o = 0; o < kOps; ++o) {
-          if (EDGE) {
-            const size_t e = ((row * p.cols) >> 3) * 8 + static_cast<size_t>(j) * 8;
-            ring_fetch<T>(dst + o * per_op * 16, plane, src[o] + e, total - e);
-          } else {
-            ring_fetch<T>(dst + o * per_op * 16, plane, src[o] + row * ld[o] + static_cast<size_t>(j) * 8);
-          }
-        }
+      for (int o = 0; o < kOps; ++o) {
+        const T* from = static_cast<const T*>(o == 0 ? p.a : o == 1 ? p.b : p.c);
+        const size_t ld = o == 0 ? p.ld_a : o == 1 ? p.ld_b : p.ld_c;
+        fetch_row<T, K, EDGE>(from, ld, row, p.rows, p.cols, j0, q.team, mask, dst + o * per_op * 16, plane);
       }
     }
     cp_async_commit();
   };
-
-  size_t ahead = at.first;
-  for (int s = 0; s < q.stages - 1; ++s, ahead += at.step) fetch(ahead, s);
-  const size_t lead = q.team < 32 ? at.first - static_cast<size_t>(at.group - (threadIdx.x & ~31) / q.team) * q.period : at.first;
-  int stage = 0, fill = q.stages - 1, buf = 0;
-  size_t row = at.first;
-  float mean = 0.f, rstd = 0.f;
-  if (row < p.rows) {
-    if (!FROM_Y) mean = __ldg(p.mean + row);
-    rstd = __ldg(p.rstd + row);
-  }
-  for (size_t go = lead; go < p.rows; go += at.step, row += at.step, buf ^= 1) {
-    float mean_next = 0.f, rstd_next = 0.f;
-    if (row + at.step < p.rows) {
-      if (!FROM_Y) mean_next = __ldg(p.mean + row + at.step);
-      rstd_next = __ldg(p.rstd + row + at.step);
+  // xhat, dy and dy * weight of one granule; zero outside the row
+  auto read = [&](const uint4* from, int k, float mean, float rstd, float2 h[4], float2 dy[4], float2 g[4]) {
+    const float4* wk = ws + k * q.team;
+    ring_read<T>(from + per_op, plane, h);
+    if (FROM_Y) {
+      get8(wk + 4 * q.chunk, q.chunk, g);
+      get8(wk + 2 * q.chunk, q.chunk, dy);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], make_float2(-g[i].x, -g[i].y)), dy[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], both(-mean)), both(rstd));
     }
-    cp_async_wait(q.stages - 2);
-    float h[K][8], dy[K][8], ds[DSUM ? K : 1][8];
-    float s1 = 0.f, s2 = 0.f;
-    const bool live = row < p.rows;
+    ring_read<T>(from, plane, dy);
+    get8(wk, q.chunk, g);
+    if (EDGE && mask[k] != 0xffu) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!((mask[k] >> (2 * i)) & 1u)) h[i].x = dy[i].x = 0.f;
+        if (!((mask[k] >> (2 * i)) & 2u)) h[i].y = dy[i].y = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[i] = mul2(g[i], dy[i]);
+  };
+
+  int row = static_cast<int>(at.first);
+  for (int s = 0; s < q.stages; ++s) fetch(row + s * step, s);
+  // the weight (with FROM_Y also 1 / weight and the bias) of the CTA's columns, granule by granule like the ring
+  if (at.group == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (mask[k] && live) {
-        const uint4* from = mine + stage * per_stage + k * q.team;
-        ring_read<T>(from, plane, dy[k]);
-        ring_read<T>(from + per_op, plane, h[k]);
-        if (DSUM) ring_read<T>(from + 2 * per_op, plane, ds[DSUM ? k : 0]);
+      if (!mask[k]) continue;
+      const long long col = static_cast<long long>(j0 + k * q.team) * 8 - at.m;
+      float v[8];
+      param8<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, v);
+      put8(ws + k * q.team, q.chunk, v);
+      if (FROM_Y) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[k][i] = FROM_Y ? (h[k][i] - b[FROM_Y ? k : 0][i]) * iw[FROM_Y ? k : 0][i] : (h[k][i] - mean) * rstd;
-        if (EDGE && mask[k] != 0xffu) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            h[k][i] = (mask[k] >> i) & 1u ? h[k][i] : 0.f;
-            dy[k][i] = (mask[k] >> i) & 1u ? dy[k][i] : 0.f;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[k][i] = dy[k][i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float g = dy[k][i] * w[k][i];
-        s1 += g;
-        s2 = fmaf(g, h[k][i], s2);
-        aw[k][i] = fmaf(dy[k][i], h[k][i], aw[k][i]);
-        ab[k][i] += dy[k][i];
+        for (int i = 0; i < 8; ++i) v[i] = 1.f / v[i];
+        put8(ws + 2 * q.chunk + k * q.team, q.chunk, v);
+        param8<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, v);
+        put8(ws + 4 * q.chunk + k * q.team, q.chunk, v);
       }
     }
-    fetch(ahead, fill);
-    ahead += at.step;
-    stage = stage + 1 == q.stages ? 0 : stage + 1;
-    fill = fill + 1 == q.stages ? 0 : fill + 1;
-
-    if (q.team <= 32) {
-      s1 = lanes_sum(s1, q.team);
-      s2 = lanes_sum(s2, q.team);
+  }
+  if (q.groups > 1) __syncthreads();   // the parameters that group 0 put down
+  // the teams of a warp shuffle together, so they leave the loop together
+  int spare = q.team < 32 ? (at.group - (threadIdx.x & ~31) / q.team) * q.period : 0;
+  float mean[kRows], rstd[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const int i = row + r * step;
+    mean[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
+    rstd[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
+  }
+  int stage = 0, buf = 0;
+  for (; row - spare < rows; row += kRows * step, buf ^= 1) {
+    // the next rows' statistics
+    float mean_next[kRows], rstd_next[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const int i = row + (kRows + r) * step;
+      mean_next[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
+      rstd_next[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
+    }
+    cp_async_wait(q.stages - kRows);
+    float s1[kRows], s2[kRows];
+    int st = stage;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float2 t1 = make_float2(0.f, 0.f), t2 = t1;
+      if (row + r * step < rows) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!mask[k]) continue;
+          float2 h[4], dy[4], g[4];
+          read(mine + st * per_stage + k * q.team, k, mean[r], rstd[r], h, dy, g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            t1 = add2(t1, g[i]);
+            t2 = fma2(g[i], h[i], t2);
+            aw[k][i] = fma2(dy[i], h[i], aw[k][i]);
+            ab[k][i] = add2(ab[k][i], dy[i]);
+          }
+        }
+      }
+      s1[r] = t1.x + t1.y;
+      s2[r] = t2.x + t2.y;
+      st = st + 1 == q.stages ? 0 : st + 1;
+    }
+    if (q.team < 32) {
+      for (int o = q.team >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          s1[r] += __shfl_xor_sync(0xffffffffu, s1[r], o);
+          s2[r] += __shfl_xor_sync(0xffffffffu, s2[r], o);
+        }
     } else {
-      s1 = warp_sum(s1);
-      s2 = warp_sum(s2);
-      const int warps = q.team >> 5, w0 = at.group * warps;
-      if ((threadIdx.x & 31) == 0) red.v[buf][threadIdx.x >> 5] = make_float4(s1, s2, 0.f, 0.f);
-      team_barrier(at.group, q.team);
-      s1 = s2 = 0.f;
-      for (int i = 0; i < warps; ++i) {
-        const float4 f = red.v[buf][w0 + i];
-        s1 += f.x;
-        s2 += f.y;
+      const float mine4 = warp_sum4(s1[0], s2[0], s1[1], s2[1]);
+      float4 f;
+      if (q.team == 32) {
+        f = make_float4(__shfl_sync(0xffffffffu, mine4, 0), __shfl_sync(0xffffffffu, mine4, 8),
+                        __shfl_sync(0xffffffffu, mine4, 16), __shfl_sync(0xffffffffu, mine4, 24));
+      } else {
+        if ((threadIdx.x & 7) == 0) reinterpret_cast<float*>(red.v[buf])[threadIdx.x >> 3] = mine4;
+        team_barrier(at.group, q.team);
+        f = gather4(red.v[buf] + at.group * (q.team >> 5), q.team >> 5);
       }
       if (CLUSTER) {
-        if (threadIdx.x < q.cluster) put_remote(&peer[buf][at.rank], threadIdx.x, make_float4(s1, s2, 0.f, 0.f));
+        if (threadIdx.x < q.cluster) put_remote(&peer[buf][at.rank], threadIdx.x, f);
         cluster_barrier();
-        s1 = s2 = 0.f;
-        for (int i = 0; i < q.cluster; ++i) {
-          s1 += peer[buf][i].x;
-          s2 += peer[buf][i].y;
-        }
+        f = gather4(peer[buf], q.cluster);
       }
+      s1[0] = f.x; s2[0] = f.y; s1[1] = f.z; s2[1] = f.w;
     }
-    s1 *= inv_n;
-    s2 *= inv_n;
-    if (live) {
-      const size_t base = EDGE ? ((row * p.cols) >> 3) * 8 : row * p.cols;
+#pragma unroll 1
+    for (int r = 0; r < kRows; ++r) {
+      const int here = row + r * step;
+      if (here < rows) {
+        const float mu = r ? mean[1] : mean[0], rs = r ? rstd[1] : rstd[0];
+        const float2 c0 = both(rs), c1 = both(-rs * ((r ? s1[1] : s1[0]) * inv_n)), c2 = both(-rs * ((r ? s2[1] : s2[0]) * inv_n));
+        const size_t base = static_cast<size_t>(here) * p.cols;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!mask[k]) continue;
-        const int j = at.rank * q.chunk + at.t + k * q.team;
-        const size_t e = base + static_cast<size_t>(j) * 8;
-        float d[8];
+        for (int k = 0; k < K; ++k) {
+          if (!mask[k]) continue;
+          const size_t e = (EDGE ? base & ~size_t(7) : base) + static_cast<size_t>(j0 + k * q.team) * 8;
+          const uint32_t keep = DROP ? keep8(__ldg(p.drop.seed), e >> 3, p.drop.stream, p.drop.last) : 0u;
+          const uint4* from = mine + stage * per_stage + k * q.team;
+          float2 h[4], dy[4], d[4];
+          read(from, k, mu, rs, h, dy, d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          d[i] = (dy[k][i] * w[k][i] - s1 - h[k][i] * s2) * rstd;
-          if (DSUM) d[i] += ds[DSUM ? k : 0][i];
-        }
-        if (EDGE) store8_masked(static_cast<T*>(p.out) + e, d, mask[k]);
-        else store8(static_cast<T*>(p.out) + e, d);
-        if (p.out2) {
-          if (p.drop.on) {
-            const uint32_t keep = keep8(key, ((row * p.cols) >> 3) + j, p.drop.stream, p.drop.last);
+          for (int i = 0; i < 4; ++i) d[i] = fma2(d[i], c0, fma2(h[i], c2, c1));     // rstd (g - mean(g) - xhat mean(g xhat))
+          if (DSUM) {
+            ring_read<T>(from + 2 * per_op, plane, h);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] = (keep >> i) & 1u ? d[i] * p.drop.scale : 0.f;
+            for (int i = 0; i < 4; ++i) d[i] = add2(d[i], h[i]);
           }
-          if (EDGE) store8_masked(static_cast<T*>(p.out2) + e, d, mask[k]);
-          else store8(static_cast<T*>(p.out2) + e, d);
+          store8_row<EDGE>(static_cast<T*>(p.out) + e, d, mask[k]);
+          if (DROP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              d[i].x = (keep >> (2 * i)) & 1u ? d[i].x * p.drop.scale : 0.f;
+              d[i].y = (keep >> (2 * i)) & 2u ? d[i].y * p.drop.scale : 0.f;
+            }
+            store8_row<EDGE>(static_cast<T*>(p.out2) + e, d, mask[k]);
+          }
         }
       }
+      fetch(here + q.stages * step, stage);     // into the slots just read for the last time
+      stage = stage + 1 == q.stages ? 0 : stage + 1;
     }
-    mean = mean_next;
-    rstd = rstd_next;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      mean[r] = mean_next[r];
+      rstd[r] = rstd_next[r];
+    }
   }
   if (CLUSTER) cluster_barrier();
   if (!partial) return;
   // the CTA's teams hold the same columns: halve their number until one is left
-  float* sums = reinterpret_cast<float*>(ring);
+  float2* sums = reinterpret_cast<float2*>(ring);
   for (int n = q.groups; n > 1;) {
-    const int low = (n + 1) / 2;
+    const int low = (n + 1) / 2, pitch = low * q.team;
     __syncthreads();
     if (at.group >= low && at.group < n) {
-      float* to = sums + (static_cast<size_t>(at.group - low) * q.team + at.t);
+      float2* to = sums + (at.group - low) * q.team + at.t;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          to[(k * 16 + i) * (low * q.team)] = aw[k][i];
-          to[(k * 16 + 8 + i) * (low * q.team)] = ab[k][i];
+        for (int i = 0; i < 4; ++i) {
+          to[(k * 8 + i) * pitch] = aw[k][i];
+          to[(k * 8 + 4 + i) * pitch] = ab[k][i];
         }
     }
     __syncthreads();
     if (at.group < n - low) {
-      const float* from = sums + (static_cast<size_t>(at.group) * q.team + at.t);
+      const float2* from = sums + at.group * q.team + at.t;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          aw[k][i] += from[(k * 16 + i) * (low * q.team)];
-          ab[k][i] += from[(k * 16 + 8 + i) * (low * q.team)];
+        for (int i = 0; i < 4; ++i) {
+          aw[k][i] = add2(aw[k][i], from[(k * 8 + i) * pitch]);
+          ab[k][i] = add2(ab[k][i], from[(k * 8 + 4 + i) * pitch]);
         }
     }
     n = low;
@@ -212,13 +241,22 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
   if (at.group == 0) {
     float* to = partial + static_cast<size_t>(blockIdx.x / q.cluster) * 2 * p.cols;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if ((mask[k] >> i) & 1u) {
-          to[col[k] + i] = aw[k][i];
-          to[p.cols + col[k] + i] = ab[k][i];
+    for (int k = 0; k < K; ++k) {
+      const long long col = static_cast<long long>(j0 + k * q.team) * 8 - at.m;
+      if (!EDGE) {
+        if (mask[k]) {
+          store8(to + col, aw[k]);
+          store8(to + p.cols + col, ab[k]);
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((mask[k] >> i) & 1u) {
+            to[col + i] = i & 1 ? aw[k][i / 2].y : aw[k][i / 2].x;
+            to[p.cols + col + i] = i & 1 ? ab[k][i / 2].y : ab[k][i / 2].x;
+          }
+      }
+    }
   }
 }
 
@@ -342,19 +380,19 @@ int column_parts(const mb_ln_desc* d) {
 }
 
 
-// Plan of the row kernel: one CTA per SM, so that there are few partials and much shared memory.
-bool plan_bwd(const mb_ln_desc* d, int ops, RowPlan* q) {
-  if (!plan_rows(d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, true, kMaxThreads, q)) return false;
-  size_grid(d->rows, 1, q);
+// Plan of the row kernel; two CTAs per SM where the registers allow.
+bool plan_bwd(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
+  if (!plan_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, true, from_y, q)) return false;
+  size_grid(d->rows, q->per_thread == 1 ? 2 : 1, q);
   return true;
 }
 
 struct Grads { void *dw, *db; float* ws; };
 
-template <typename T, int K, bool FROM_Y, bool DSUM, bool EDGE, bool CLUSTER>
+template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
 int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
   static std::atomic<int> cache[64];
-  auto kernel = ln_bwd_rows<T, K, FROM_Y, DSUM, EDGE, CLUSTER>;
+  auto kernel = ln_bwd_rows<T, K, FROM_Y, DSUM, DROP, EDGE, CLUSTER>;
   int regs = 0;
   if (int rc = prepare("layer_norm_bwd", kernel, cache, &regs)) return rc;
   fit_clusters(kernel, &q);
@@ -363,20 +401,25 @@ int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
   return sums ? finish<T>(g.ws, q.grid / q.cluster, p.cols, g.dw, g.db, p.w_f32, st) : MB_OK;
 }
 
-template <typename T, bool FROM_Y, bool DSUM, bool EDGE>
+template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
 int pick_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
-  if (q.cluster > 1) return launch_bwd<T, 2, FROM_Y, DSUM, EDGE, true>(p, q, g, st);
-  if (q.per_thread == 1) return launch_bwd<T, 1, FROM_Y, DSUM, EDGE, false>(p, q, g, st);
-  return launch_bwd<T, 2, FROM_Y, DSUM, EDGE, false>(p, q, g, st);
+  if (q.cluster > 1) return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, true>(p, q, g, st);
+  if (q.per_thread == 1) return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+  return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+}
+
+template <typename T, bool FROM_Y, bool DSUM, bool DROP>
+int pick_edge(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
+  return p.cols % 8 ? pick_bwd<T, FROM_Y, DSUM, DROP, true>(p, q, g, st) : pick_bwd<T, FROM_Y, DSUM, DROP, false>(p, q, g, st);
 }
 
 template <typename T, bool FROM_Y>
 int bwd(const LnArgs& p, const mb_ln_desc* d, bool granules, const Grads& g, cudaStream_t st) {
   RowPlan q;
-  if (granules && plan_bwd(d, p.c ? 3 : 2, &q)) {
-    const bool edge = p.cols % 8 != 0;
-    if (p.c) return edge ? pick_bwd<T, FROM_Y, true, true>(p, q, g, st) : pick_bwd<T, FROM_Y, true, false>(p, q, g, st);
-    return edge ? pick_bwd<T, FROM_Y, false, true>(p, q, g, st) : pick_bwd<T, FROM_Y, false, false>(p, q, g, st);
+  // (a dx that equals dv because nothing is dropped is rare enough for the element-wise kernels)
+  if (granules && (p.drop.on || !p.out2) && plan_bwd(d, p.c ? 3 : 2, FROM_Y, &q)) {
+    if (p.drop.on) return p.c ? pick_edge<T, FROM_Y, true, true>(p, q, g, st) : pick_edge<T, FROM_Y, false, true>(p, q, g, st);
+    return p.c ? pick_edge<T, FROM_Y, true, false>(p, q, g, st) : pick_edge<T, FROM_Y, false, false>(p, q, g, st);
   }
   if (g.dw || g.db) {      // before the outputs, which may lie over the inputs
     const int parts = column_parts(d);
@@ -400,8 +443,8 @@ size_t mb_layer_norm_workspace_bytes(const mb_ln_desc* d) {
   // which kernel runs also depends on addresses: enough for any
   int parts = column_parts(d);
   RowPlan q;
-  for (int ops = 2; ops <= 3; ++ops)
-    if (plan_bwd(d, ops, &q) && q.grid / q.cluster > parts) parts = q.grid / q.cluster;
+  for (int form = 0; form < 4; ++form)
+    if (plan_bwd(d, 2 + form / 2, form % 2, &q) && q.grid / q.cluster > parts) parts = q.grid / q.cluster;
   return static_cast<size_t>(parts) * 2 * d->cols * sizeof(float);
 }
 

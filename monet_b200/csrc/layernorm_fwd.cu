@@ -41,7 +41,7 @@ __device__ __forceinline__ void combine_stats(WarpSums& red, float4 (*peer)[8], 
 }
 
 template <typename T, int K, bool RES, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
+__global__ void __launch_bounds__(kMaxTeam) ln_fwd_rows(LnArgs p, RowPlan q) {
   extern __shared__ __align__(128) uint4 ring[];
   if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
   __shared__ WarpSums red;
@@ -253,7 +253,7 @@ int pick_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
 template <typename T>
 int fwd(const LnArgs& p, bool granules, cudaStream_t st) {
   RowPlan q;
-  if (granules && plan_rows(p.cols, sizeof(T), p.b ? 2 : 1, false, 256, &q)) {
+  if (granules && plan_rows(p.rows, p.cols, sizeof(T), p.b ? 2 : 1, false, false, &q)) {
     const bool edge = p.cols % 8 != 0;
     if (p.b) return edge ? pick_fwd<T, true, true>(p, q, st) : pick_fwd<T, true, false>(p, q, st);
     return edge ? pick_fwd<T, false, true>(p, q, st) : pick_fwd<T, false, false>(p, q, st);

@@ -54,6 +54,20 @@ __device__ __forceinline__ uint4 philox(unsigned long long key, unsigned long lo
   return make_uint4(c0, c1, c2, c3);
 }
 
+// The ties of a block, decided by the lower halves: one block in 8192, so it is kept out of line.
+static __device__ __noinline__ uint32_t keep8_ties(unsigned long long key, unsigned long long block, uint32_t stream, uint32_t last,
+                                            uint4 q) {
+  const uint4 s = philox(key, block, stream, 1);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w}, v[4] = {s.x, s.y, s.z, s.w};
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t hi = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu, lo = (v[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+    if (hi == (last >> 16) && lo > (last & 0xffffu)) keep |= 1u << j;
+  }
+  return keep;
+}
+
 // Bit j of the result: element 8 * block + j is kept.
 __device__ __forceinline__ uint32_t keep8(unsigned long long key, unsigned long long block, uint32_t stream, uint32_t last) {
   const uint4 q = philox(key, block, stream, 0);
@@ -69,15 +83,7 @@ __device__ __forceinline__ uint32_t keep8(unsigned long long key, unsigned long 
     tie |= (x - 0x10001u) & ~x & 0x80008000u;
   }
   // `tie` is non-zero exactly when one of the eight halves ties
-  if (tie && (last & 0xffffu) != 0xffffu) {
-    const uint4 s = philox(key, block, stream, 1);
-    const uint32_t v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t hi = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu, lo = (v[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-      if (hi == (last >> 16) && lo > (last & 0xffffu)) keep |= 1u << j;
-    }
-  }
+  if (tie && (last & 0xffffu) != 0xffffu) keep |= keep8_ties(key, block, stream, last, q);
   return keep;
 }
 
