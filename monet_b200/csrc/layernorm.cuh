@@ -29,13 +29,6 @@ struct LnArgs {
   Drop drop;
 };
 
-// ---- rows in registers ---------------------------------------------------------------------
-// A team of threads (part of a warp up to a cluster of CTAs) holds a row in registers: it is read
-// once, its statistics are formed from the registers, and the result is written.  Rows to come are
-// fetched by asynchronous copies meanwhile (rows.cuh).
-
-struct WarpSums { float4 v[2][kMaxThreads / 32]; };   // double-buffered by row: one barrier a row
-
 // ---- any shape, any stride, any alignment ----------------------------------------------------
 // One CTA per row, element-wise accesses; a row is read again for each of its three uses, from L2
 // when it is long.
@@ -53,57 +46,113 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-// A row stays in registers when it fits kMaxTeam * K granules per CTA and eight CTAs, K being at
-// most 4 (8 in a cluster) forward and 2 backward, where each value also has two column sums and a
-// weight; longer rows, and tensors whose rows do not lie on granule boundaries in the same way, take
-// the element-wise kernels.
-constexpr int kRingLimit = 216 * 1024;
+// Rows whose tensors lie on granule boundaries in the same way are walked in granules (rows.cuh), one
+// thread holding up to 16 values (32 forward, where there are no column sums) and a team up to
+// kMaxTeam threads.  Longer rows: forward stays in the shared memory of up to eight CTAs, backward in
+// the registers of up to eight.  Everything else takes the element-wise kernels.
+constexpr size_t kSmemLimit = 216 * 1024;
 
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+// Rows between two barriers of the backward kernel with k granules a thread.
+constexpr int bwd_rows_between_barriers(int k) { return k == 1 ? 2 : 1; }
+constexpr int fwd_rows_between_barriers(int k, int elems) { return k * elems <= 16 ? 2 : 1; }
 
-inline bool plan_rows(size_t rows, size_t cols, int elem, int ops, bool backward, bool from_y, RowPlan* q) {
-  if (rows >> 30) return false;                              // row numbers are 32-bit, and some steps ahead
-  int g = 8;
-  while (cols % g) g /= 2;                                   // gcd(cols, 8)
-  q->period = 8 / g;
-  const size_t most = (cols + (8 - g) + 7) / 8;              // granules a row can touch
-  const int k_max = backward ? 2 : 4, k_cluster = backward ? 2 : 8;
-  if (most > static_cast<size_t>(kMaxTeam) * 8 * k_cluster) return false;
-  for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
-    q->chunk = ceil_div(static_cast<long long>(most), q->cluster);
-    if (q->chunk > kMaxTeam * (q->cluster == 8 ? k_cluster : k_max)) continue;
-    if (q->chunk <= 32) {
-      q->team = 1;
-      while (q->team < q->chunk) q->team *= 2;
-      q->per_thread = 1;
-    } else {
-      const int wish = backward ? 256 : 128;
-      int k = 1;
-      while (k < k_max && ceil_div(q->chunk, 32 * k) * 32 > wish) k *= 2;
-      while (ceil_div(q->chunk, 32 * k) * 32 > kMaxTeam) k *= 2;
-      q->per_thread = k;
-      q->team = ceil_div(q->chunk, 32 * k) * 32;
-    }
-    const int threads = !backward ? 256 : q->per_thread == 1 ? 512 : 768;
-    q->groups = q->cluster > 1 || q->team >= threads ? 1 : threads / q->team;
-    if (q->team > 32 && q->groups > 15) q->groups = 15;      // named barriers
-    const size_t stage = static_cast<size_t>(q->groups) * q->chunk * 8 * elem * ops;
-    if (backward) {
-      // two CTAs per SM of one granule a thread; fp32 weight (and its inverse and the bias) beside the ring
-      const size_t params = static_cast<size_t>(q->chunk) * 32 * (from_y ? 3 : 1);
-      const size_t budget = (q->per_thread == 1 ? 104 : 208) * 1024;
-      const int deep = budget > params ? static_cast<int>((budget - params) / stage) : 0;
-      q->stages = deep > 8 ? 8 : deep < kRows ? kRows : deep;
-      q->smem = stage * q->stages + params;
-      const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * 16 * sizeof(float) : 0;
-      if (fold > q->smem) q->smem = fold;                    // the teams' column sums are folded there
-    } else {
-      const int deep = static_cast<int>(64 * 1024 / stage);
-      q->stages = deep > 6 ? 6 : deep < 2 ? 2 : deep;
-      q->smem = stage * q->stages;
-    }
-    if (q->smem <= kRingLimit) return true;
+// The period of the rows' alignment, and the granules that a row can touch.
+inline size_t row_granules(size_t cols, int elems, int* period) {
+  int g = elems;
+  while (cols % g) g /= 2;
+  *period = elems / g;
+  return (cols + (elems - g) + elems - 1) / elems;
+}
+
+// Threads for `chunk` granules of up to `most` a thread; false if they do not fit a team.
+inline bool plan_team(int chunk, int most, RowPlan* q) {
+  q->chunk = chunk;
+  q->per_thread = 1;
+  if (chunk <= 32) {                   // several rows a warp, or one
+    for (q->team = 1; q->team < chunk;) q->team *= 2;
+    return true;
   }
+  while (q->per_thread < most && chunk > 32 * q->per_thread) q->per_thread *= 2;    // one warp if possible: no barrier
+  q->team = ceil_div(chunk, 32 * q->per_thread) * 32;
+  return q->team <= kMaxTeam;
+}
+
+// Teams per CTA: as many as `threads` hold, fewer where the rows would not reach every SM.
+inline void plan_groups(size_t rows, int threads, RowPlan* q) {
+  q->groups = q->cluster > 1 ? 1 : threads / q->team;
+  if (q->team > 32 && q->groups > 15) q->groups = 15;        // named barriers
+  const size_t spread = (rows + num_sms() - 1) / num_sms();
+  if (static_cast<size_t>(q->groups) > spread) q->groups = static_cast<int>(spread);
+  if (q->groups < 1) q->groups = 1;
+  if (q->team < 32) q->groups = (q->groups + 32 / q->team - 1) / (32 / q->team) * (32 / q->team);    // whole warps
+}
+
+inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from_y, RowPlan* q) {
+  if (rows >> 30) return false;                              // row numbers are 32-bit, and some steps ahead
+  const int elems = 16 / elem;
+  const size_t most = row_granules(cols, elems, &q->period);
+  if (most > static_cast<size_t>(kMaxTeam) * 8 * (16 / elems)) return false;
+  for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
+    if (!plan_team(ceil_div(most, q->cluster), 16 / elems, q)) continue;
+    if (q->cluster > 1) {                                    // the cluster's kernel has 16 values a thread
+      q->per_thread = 16 / elems;
+      q->team = ceil_div(q->chunk, 32 * q->per_thread) * 32;
+    }
+    plan_groups(rows, kMaxThreads, q);
+    // one CTA per SM; the fp32 weight (with from_y its inverse and the bias) beside the ring
+    const int r = bwd_rows_between_barriers(q->per_thread);
+    const size_t stage = static_cast<size_t>(q->groups * q->team / 32) * q->per_thread * ops * kUnit;
+    const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 4 * (from_y ? 3 : 1);
+    const size_t deep = (kSmemLimit - params) / (r * stage);
+    if (deep < 2) continue;
+    q->stages = r * static_cast<int>(deep > 8 / r ? 8 / r : deep);
+    q->smem = stage * q->stages + params;
+    const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
+    if (fold > q->smem) q->smem = fold;                      // the teams' column sums are folded there
+    return q->smem <= kSmemLimit;
+  }
+  return false;
+}
+
+inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* q) {
+  if (rows >> 30) return false;
+  const int elems = 16 / elem;
+  const size_t most = row_granules(cols, elems, &q->period);
+  q->cluster = 1;
+  if (most > static_cast<size_t>(kMaxTeam) * (32 / elems)) return false;
+  if (!plan_team(static_cast<int>(most), 16 / elems, q)) {
+    q->per_thread = 32 / elems;
+    q->team = ceil_div(static_cast<int>(most), 32 * q->per_thread) * 32;
+  }
+  plan_groups(rows, kMaxThreads, q);
+  const int r = fwd_rows_between_barriers(q->per_thread, elems);
+  const size_t stage = static_cast<size_t>(q->groups * q->team / 32) * q->per_thread * ops * kUnit;
+  const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
+  const size_t budget = (q->groups * q->team > kMaxThreads / 2 ? kSmemLimit : 100 * 1024) - params;
+  const size_t deep = budget / (r * stage);
+  if (deep < 1) return false;
+  q->stages = r * static_cast<int>(deep > 8 / r ? 8 / r : deep);
+  q->smem = stage * q->stages + params;
+  return true;
+}
+
+// One row in the shared memory of 1 to 8 CTAs, of which two share an SM if they are small enough.
+inline bool plan_fwd_long(size_t rows, size_t cols, int elem, int ops, RowPlan* q) {
+  if (rows >> 30) return false;
+  const size_t most = row_granules(cols, 16 / elem, &q->period);
+  for (size_t limit = 106 * 1024; limit <= kSmemLimit; limit += kSmemLimit - 106 * 1024)
+    for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
+      const size_t chunk = (most + q->cluster - 1) / q->cluster;
+      if (chunk > 65536) continue;
+      q->chunk = static_cast<int>(chunk);
+      q->team = kMaxTeam;
+      q->groups = 1;
+      q->stages = 1;
+      q->per_thread = ceil_div(q->chunk, q->team);
+      q->smem = static_cast<size_t>(q->team) / 32 * q->per_thread * ops * kUnit;
+      if (q->smem <= limit) return true;
+    }
   return false;
 }
 
@@ -128,7 +177,7 @@ int prepare(const char* who, Kernel kernel, std::atomic<int>* cache, int* regs) 
   int r = cache[dev].load(std::memory_order_relaxed);
   if (r == 0) {
     cudaFuncAttributes a;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLimit);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return fail(MB_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(cudaGetLastError()));
     r = a.numRegs + 1;
@@ -202,12 +251,13 @@ bool natural(const mb_ln_desc* d, const void* p) { return aligned(p, dtype_bytes
 bool natural_param(const mb_ln_desc* d, const void* p) { return aligned(p, dtype_bytes(d->param_dtype)); }
 
 
-// Whether every tensor's rows lie on granule boundaries in the same way.
+// Whether every tensor's rows (address, row stride) lie on granule boundaries in the same way.
 inline bool on_granules(const mb_ln_desc* d, std::initializer_list<std::pair<const void*, size_t>> tensors) {
   for (const auto& t : tensors) {
     if (!t.first) continue;
-    if (!aligned(t.first, 8 * dtype_bytes(d->dtype))) return false;
-    if (d->cols % 8 ? t.second != d->cols : t.second % 8 != 0) return false;
+    const size_t elems = 16 / dtype_bytes(d->dtype);
+    if (!aligned(t.first, 16)) return false;
+    if (d->cols % elems ? t.second != d->cols : t.second % elems != 0) return false;
   }
   return true;
 }

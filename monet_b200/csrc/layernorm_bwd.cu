@@ -6,210 +6,246 @@ namespace {
 
 // Backward.  partial[team CTA][0][col] = sum of dy xhat, [1][col] = sum of dy over the CTA's rows.
 //
-// kRows rows are handled between two barriers: their sums (mean(g), mean(g xhat)) are formed from a
-// first reading of the ring, then the rows are read a second time to form dv.  Reading twice costs
-// shared-memory loads but no registers, which the column sums need; the parameters lie in shared
-// memory for the same reason.  With 64 registers a thread two CTAs share an SM, and one computes
-// while the other waits for its barrier.
-template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(K == 1 ? kMaxTeam : kMaxThreads, K == 1 ? 2 : 1) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
+// R rows are handled between two barriers: their sums are formed from a first reading of the
+// ring, then the rows are read a second time to form dv.  Reading twice costs shared-memory loads but
+// no registers, which the column sums need; the parameters lie in shared memory for the same reason
+// (in registers where a thread has one granule).  With 80 registers a thread, 24 warps share an SM,
+// and one team computes while another waits for its barrier.
+//
+// With t = v - mean or y - b:  sum g xhat = rstd sum (dy t) w  or  sum dy t  (the weight cancels), and
+// dw = sum over rows of (dy t) rstd  or  (sum dy t) / w, so xhat itself is never formed.
+template <typename T, int K, int R, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
+__global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
+  __shared__ float red[2][kMaxThreads / 32][2 * R];      // double-buffered by row: one barrier a row
+  __shared__ float peer[2][8][2 * R];
   if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
-  __shared__ WarpSums red;
-  __shared__ float4 peer[2][8];
-  constexpr int kOps = DSUM ? 3 : 2;
-  const RowWalk at(q, static_cast<int>(p.cols));
-  const int granules = EDGE ? static_cast<int>((at.m + p.cols + 7) >> 3) : static_cast<int>(p.cols >> 3);
+  constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 3 : 1;
+  constexpr int kParam = kParamUnits<T> * kUnit;
+  constexpr bool kInRegs = K == 1;
+  const RowWalk at(q, p.cols, E);
   const float inv_n = 1.f / static_cast<float>(p.cols);
   const int j0 = at.rank * q.chunk + at.t;           // the thread's granules: j0 + k * team
-  const int rows = static_cast<int>(p.rows), step = static_cast<int>(at.step);
+  const int rows = static_cast<int>(p.rows), step = at.step;
+  const uint32_t stride = (blockDim.x >> 5) * (kSlots * kUnit);      // a stage
+  const uint32_t slots = sm100::smem_u32(ring) + (threadIdx.x >> 5) * (kSlots * kUnit) + (threadIdx.x & 31) * 16;
+  const uint32_t params = sm100::smem_u32(ring) + q.stages * stride + (at.t >> 5) * (K * kKinds * kParam) + (at.t & 31) * 16;
+  const uint32_t kstep = q.team * 16;
 
   uint32_t mask[K];
-  float2 aw[K][4], ab[K][4];
+  float2 aw[K][P], ab[K][P];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    mask[k] = column_mask<EDGE>(at, q, granules, static_cast<int>(p.cols), k);
+    mask[k] = column_mask<T, EDGE>(at, q, at.t + k * q.team, p.cols);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) aw[k][i] = ab[k][i] = make_float2(0.f, 0.f);
+    for (int i = 0; i < P; ++i) aw[k][i] = ab[k][i] = both(0.f);
   }
 
-  const int plane = q.chunk;
-  const int per_op = plane * kPlanes<T>, per_stage = per_op * kOps;
-  uint4* mine = ring + at.group * q.stages * per_stage + at.t;
-  float4* const ws = reinterpret_cast<float4*>(ring) + q.stages * q.groups * per_stage + at.t;
-
-  auto fetch = [&](int row, int stage) {
-    if (row < rows) {
-      const uint32_t dst = sm100::smem_u32(mine) + stage * per_stage * 16;
+  // byte offset of the thread's first granule in the first of the rows at hand (all tensors are dense)
+  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, j0) * sizeof(T);
+  const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
+  auto fetch = [&](uint32_t stage, size_t off) {
 #pragma unroll
-      for (int o = 0; o < kOps; ++o) {
-        const T* from = static_cast<const T*>(o == 0 ? p.a : o == 1 ? p.b : p.c);
-        const size_t ld = o == 0 ? p.ld_a : o == 1 ? p.ld_b : p.ld_c;
-        fetch_row<T, K, EDGE>(from, ld, row, p.rows, p.cols, j0, q.team, mask, dst + o * per_op * 16, plane);
-      }
+    for (int o = 0; o < kOps; ++o)
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (mask[k]) ring_copy<EDGE>(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, p.rows * p.cols * sizeof(T));
+  };
+
+  float2 wr[P], nbr[P], iwr[P];        // kInRegs: the weight; with FROM_Y minus the bias and 1 / weight
+  auto weight = [&](int k, float2 v[P]) {
+    if constexpr (kInRegs) copy_pairs(wr, v); else param_get<T>(params + (k * kKinds) * kParam, v);
+  };
+  auto minus_bias = [&](int k, float2 v[P]) {
+    if constexpr (kInRegs) copy_pairs(nbr, v); else param_get<T>(params + (k * kKinds + 1) * kParam, v);
+  };
+  auto inverse_weight = [&](int k, float2 v[P]) {
+    if constexpr (kInRegs) copy_pairs(iwr, v); else param_get<T>(params + (k * kKinds + 2) * kParam, v);
+  };
+  // t and dy of one granule; zero outside the row
+  auto read = [&](uint32_t stage, int k, float mean, float2 (&t)[P], float2 (&dy)[P]) {
+    ring_get<T>(stage + (k * kOps + 1) * kUnit, t);
+    if (FROM_Y) minus_bias(k, dy);
+#pragma unroll
+    for (int i = 0; i < P; ++i) t[i] = add2(t[i], FROM_Y ? dy[i] : both(-mean));
+    ring_get<T>(stage + (k * kOps) * kUnit, dy);
+    if (EDGE && mask[k] != (1u << E) - 1) {
+      zero_outside(t, mask[k]);
+      zero_outside(dy, mask[k]);
     }
+  };
+
+  // slots that are never fetched hold zeros, so that the sums need not ask
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (!mask[k])
+      for (int s = 0; s < q.stages; ++s)
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) smem_put(slots + s * stride + (k * kOps + o) * kUnit, make_uint4(0, 0, 0, 0));
+  for (int s = 0; s < q.stages; s += R) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (at.first + (s + r) * step < rows) fetch(slots + (s + r) * stride, out + (s + r) * out_step);
     cp_async_commit();
-  };
-  // xhat, dy and dy * weight of one granule; zero outside the row
-  auto read = [&](const uint4* from, int k, float mean, float rstd, float2 h[4], float2 dy[4], float2 g[4]) {
-    const float4* wk = ws + k * q.team;
-    ring_read<T>(from + per_op, plane, h);
-    if (FROM_Y) {
-      get8(wk + 4 * q.chunk, q.chunk, g);
-      get8(wk + 2 * q.chunk, q.chunk, dy);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], make_float2(-g[i].x, -g[i].y)), dy[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = mul2(add2(h[i], both(-mean)), both(rstd));
-    }
-    ring_read<T>(from, plane, dy);
-    get8(wk, q.chunk, g);
-    if (EDGE && mask[k] != 0xffu) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!((mask[k] >> (2 * i)) & 1u)) h[i].x = dy[i].x = 0.f;
-        if (!((mask[k] >> (2 * i)) & 2u)) h[i].y = dy[i].y = 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[i] = mul2(g[i], dy[i]);
-  };
-
-  int row = static_cast<int>(at.first);
-  for (int s = 0; s < q.stages; ++s) fetch(row + s * step, s);
-  // the weight (with FROM_Y also 1 / weight and the bias) of the CTA's columns, granule by granule like the ring
-  if (at.group == 0) {
+  }
+  if (kInRegs || at.group == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (!mask[k]) continue;
-      const long long col = static_cast<long long>(j0 + k * q.team) * 8 - at.m;
-      float v[8];
-      param8<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, v);
-      put8(ws + k * q.team, q.chunk, v);
+      const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
+      float2 v[P];
+      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, v);
+      if constexpr (kInRegs) copy_pairs(v, wr); else param_put<T>(params + (k * kKinds) * kParam, v);
       if (FROM_Y) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 1.f / v[i];
-        put8(ws + 2 * q.chunk + k * q.team, q.chunk, v);
-        param8<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, v);
-        put8(ws + 4 * q.chunk + k * q.team, q.chunk, v);
+        for (int i = 0; i < P; ++i) v[i] = make_float2(1.f / v[i].x, 1.f / v[i].y);
+        if constexpr (kInRegs) copy_pairs(v, iwr); else param_put<T>(params + (k * kKinds + 2) * kParam, v);
+        load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, v);
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = make_float2(-v[i].x, -v[i].y);
+        if constexpr (kInRegs) copy_pairs(v, nbr); else param_put<T>(params + (k * kKinds + 1) * kParam, v);
       }
     }
   }
-  if (q.groups > 1) __syncthreads();   // the parameters that group 0 put down
-  // the teams of a warp shuffle together, so they leave the loop together
-  int spare = q.team < 32 ? (at.group - (threadIdx.x & ~31) / q.team) * q.period : 0;
-  float mean[kRows], rstd[kRows];
+  if (!kInRegs && q.groups > 1) __syncthreads();   // the parameters that group 0 put down
+
+  int row = at.first;
+  const int spare = at.spare(q);
+  float mean[R], rstd[R];
+  auto statistics = [&](int first, float (&m)[R], float (&s)[R]) {
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const int i = row + r * step;
-    mean[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
-    rstd[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
-  }
-  int stage = 0, buf = 0;
-  for (; row - spare < rows; row += kRows * step, buf ^= 1) {
-    // the next rows' statistics
-    float mean_next[kRows], rstd_next[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int i = row + (kRows + r) * step;
-      mean_next[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
-      rstd_next[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
+    for (int r = 0; r < R; ++r) {
+      const int i = first + r * step;
+      m[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
+      s[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
     }
-    cp_async_wait(q.stages - kRows);
-    float s1[kRows], s2[kRows];
-    int st = stage;
+  };
+  statistics(row, mean, rstd);
+  uint32_t stage = slots;
+  int buf = 0;
+  for (; row - spare < rows; row += R * step, buf ^= 1) {
+    float mean_next[R], rstd_next[R];
+    statistics(row + R * step, mean_next, rstd_next);
+    cp_async_wait(q.stages / R - 1);
+    float2 t1[R], t2[R];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      float2 t1 = make_float2(0.f, 0.f), t2 = t1;
-      if (row + r * step < rows) {
+    for (int r = 0; r < R; ++r) t1[r] = t2[r] = both(0.f);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (!mask[k]) continue;
-          float2 h[4], dy[4], g[4];
-          read(mine + st * per_stage + k * q.team, k, mean[r], rstd[r], h, dy, g);
+    for (int k = 0; k < K; ++k) {
+      float2 w[P];
+      weight(k, w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            t1 = add2(t1, g[i]);
-            t2 = fma2(g[i], h[i], t2);
-            aw[k][i] = fma2(dy[i], h[i], aw[k][i]);
-            ab[k][i] = add2(ab[k][i], dy[i]);
+      for (int r = 0; r < R; ++r) {
+        if (row + r * step >= rows) continue;
+        float2 t[P], dy[P];
+        read(stage + r * stride, k, mean[r], t, dy);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const float2 u = mul2(dy[i], t[i]);
+          t1[r] = fma2(dy[i], w[i], t1[r]);
+          ab[k][i] = add2(ab[k][i], dy[i]);
+          if (FROM_Y) {
+            t2[r] = add2(t2[r], u);
+            aw[k][i] = add2(aw[k][i], u);
+          } else {
+            t2[r] = fma2(u, w[i], t2[r]);
+            aw[k][i] = fma2(u, both(rstd[r]), aw[k][i]);
           }
         }
       }
-      s1[r] = t1.x + t1.y;
-      s2[r] = t2.x + t2.y;
-      st = st + 1 == q.stages ? 0 : st + 1;
     }
-    if (q.team < 32) {
-      for (int o = q.team >> 1; o > 0; o >>= 1)
+    float s[2 * R];                      // sum dy w and sum g t of each row
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          s1[r] += __shfl_xor_sync(0xffffffffu, s1[r], o);
-          s2[r] += __shfl_xor_sync(0xffffffffu, s2[r], o);
-        }
+    for (int r = 0; r < R; ++r) {
+      s[2 * r] = t1[r].x + t1[r].y;
+      s[2 * r + 1] = t2[r].x + t2[r].y;
+    }
+    if (q.team <= 32) {
+      lanes_sums(s, q.team);
     } else {
-      const float mine4 = warp_sum4(s1[0], s2[0], s1[1], s2[1]);
-      float4 f;
-      if (q.team == 32) {
-        f = make_float4(__shfl_sync(0xffffffffu, mine4, 0), __shfl_sync(0xffffffffu, mine4, 8),
-                        __shfl_sync(0xffffffffu, mine4, 16), __shfl_sync(0xffffffffu, mine4, 24));
-      } else {
-        if ((threadIdx.x & 7) == 0) reinterpret_cast<float*>(red.v[buf])[threadIdx.x >> 3] = mine4;
-        team_barrier(at.group, q.team);
-        f = gather4(red.v[buf] + at.group * (q.team >> 5), q.team >> 5);
-      }
+      const float x = warp_sums(s);
+      if ((threadIdx.x & (16 / R - 1)) == 0) red[buf][threadIdx.x >> 5][(threadIdx.x & 31) / (16 / R)] = x;
+      team_barrier(at.group, q.team);
+      gather(red[buf][at.group * (q.team >> 5)], q.team >> 5, s);
       if (CLUSTER) {
-        if (threadIdx.x < q.cluster) put_remote(&peer[buf][at.rank], threadIdx.x, f);
+        if (threadIdx.x < q.cluster)
+#pragma unroll
+          for (int i = 0; i < 2 * R; ++i) put_remote(&peer[buf][at.rank][i], threadIdx.x, s[i]);
         cluster_barrier();
-        f = gather4(peer[buf], q.cluster);
+        gather(peer[buf][0], q.cluster, s);
       }
-      s1[0] = f.x; s2[0] = f.y; s1[1] = f.z; s2[1] = f.w;
     }
+    uint32_t keep[K];
+    if (DROP) {
+      const unsigned long long key = __ldg(p.drop.seed);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        keep[k] = 0;
 #pragma unroll 1
-    for (int r = 0; r < kRows; ++r) {
-      const int here = row + r * step;
-      if (here < rows) {
-        const float mu = r ? mean[1] : mean[0], rs = r ? rstd[1] : rstd[0];
-        const float2 c0 = both(rs), c1 = both(-rs * ((r ? s1[1] : s1[0]) * inv_n)), c2 = both(-rs * ((r ? s2[1] : s2[0]) * inv_n));
-        const size_t base = static_cast<size_t>(here) * p.cols;
+        for (int r = R - 1; r >= 0; --r) keep[k] = keep[k] << E | keep_granule<T>(p.drop, key, (out + r * out_step + k * kstep) / 16);
+      }
+    }
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          if (!mask[k]) continue;
-          const size_t e = (EDGE ? base & ~size_t(7) : base) + static_cast<size_t>(j0 + k * q.team) * 8;
-          const uint32_t keep = DROP ? keep8(__ldg(p.drop.seed), e >> 3, p.drop.stream, p.drop.last) : 0u;
-          const uint4* from = mine + stage * per_stage + k * q.team;
-          float2 h[4], dy[4], d[4];
-          read(from, k, mu, rs, h, dy, d);
+    for (int k = 0; k < K; ++k) {
+      float2 w[P];
+      weight(k, w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[i] = fma2(d[i], c0, fma2(h[i], c2, c1));     // rstd (g - mean(g) - xhat mean(g xhat))
-          if (DSUM) {
-            ring_read<T>(from + 2 * per_op, plane, h);
+      for (int r = 0; r < R; ++r) {
+        if (row + r * step >= rows) continue;
+        // rstd (g - mean(g) - xhat mean(g xhat))
+        const float2 c1 = both(-s[2 * r] * inv_n), c2 = both(FROM_Y ? -s[2 * r + 1] * inv_n : -s[2 * r + 1] * inv_n * rstd[r] * rstd[r]);
+        float2 t[P], d[P];
+        read(stage + r * stride, k, mean[r], t, d);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = add2(d[i], h[i]);
-          }
-          store8_row<EDGE>(static_cast<T*>(p.out) + e, d, mask[k]);
-          if (DROP) {
+        for (int i = 0; i < P; ++i) d[i] = fma2(d[i], w[i], c1);
+        if (FROM_Y) {
+          float2 iw[P];
+          inverse_weight(k, iw);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              d[i].x = (keep >> (2 * i)) & 1u ? d[i].x * p.drop.scale : 0.f;
-              d[i].y = (keep >> (2 * i)) & 2u ? d[i].y * p.drop.scale : 0.f;
-            }
-            store8_row<EDGE>(static_cast<T*>(p.out2) + e, d, mask[k]);
-          }
+          for (int i = 0; i < P; ++i) t[i] = mul2(t[i], iw[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) d[i] = fma2(t[i], c2, d[i]);
+        if (DSUM) {
+          ring_get<T>(stage + r * stride + (k * kOps + 2) * kUnit, t);
+#pragma unroll
+          for (int i = 0; i < P; ++i) d[i] = fma2(d[i], both(rstd[r]), t[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < P; ++i) d[i] = mul2(d[i], both(rstd[r]));
+        }
+        const size_t e = out + r * out_step + k * kstep;
+        if (mask[k]) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), d, mask[k]);
+        if (DROP) {
+          apply_keep(d, keep[k] >> (E * r), p.drop.scale);
+          if (mask[k]) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out2) + e), d, mask[k]);
         }
       }
-      fetch(here + q.stages * step, stage);     // into the slots just read for the last time
-      stage = stage + 1 == q.stages ? 0 : stage + 1;
     }
+    // the next rows into the slots just read for the last time
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
+    for (int r = 0; r < R; ++r)
+      if (row + (q.stages + r) * step < rows) fetch(stage + r * stride, out + (q.stages + r) * out_step);
+    cp_async_commit();
+    stage += R * stride;
+    if (stage >= slots + q.stages * stride) stage = slots;
+    out += R * out_step;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       mean[r] = mean_next[r];
       rstd[r] = rstd_next[r];
     }
   }
-  if (CLUSTER) cluster_barrier();
+  if (CLUSTER) cluster_barrier();      // no CTA leaves while a peer may still write into it
   if (!partial) return;
+  if (FROM_Y) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float2 iw[P];
+      inverse_weight(k, iw);
+#pragma unroll
+      for (int i = 0; i < P; ++i) aw[k][i] = mul2(aw[k][i], iw[i]);
+    }
+  }
   // the CTA's teams hold the same columns: halve their number until one is left
   float2* sums = reinterpret_cast<float2*>(ring);
   for (int n = q.groups; n > 1;) {
@@ -220,20 +256,20 @@ __global__ void __launch_bounds__(K == 1 ? kMaxTeam : kMaxThreads, K == 1 ? 2 : 
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          to[(k * 8 + i) * pitch] = aw[k][i];
-          to[(k * 8 + 4 + i) * pitch] = ab[k][i];
+        for (int i = 0; i < P; ++i) {
+          to[(k * 2 * P + i) * pitch] = aw[k][i];
+          to[(k * 2 * P + P + i) * pitch] = ab[k][i];
         }
     }
     __syncthreads();
     if (at.group < n - low) {
-      const float2* from = sums + at.group * q.team + at.t;
+      const float2* have = sums + at.group * q.team + at.t;
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          aw[k][i] = add2(aw[k][i], from[(k * 8 + i) * pitch]);
-          ab[k][i] = add2(ab[k][i], from[(k * 8 + 4 + i) * pitch]);
+        for (int i = 0; i < P; ++i) {
+          aw[k][i] = add2(aw[k][i], have[(k * 2 * P + i) * pitch]);
+          ab[k][i] = add2(ab[k][i], have[(k * 2 * P + P + i) * pitch]);
         }
     }
     n = low;
@@ -242,18 +278,20 @@ __global__ void __launch_bounds__(K == 1 ? kMaxTeam : kMaxThreads, K == 1 ? 2 : 
     float* to = partial + static_cast<size_t>(blockIdx.x / q.cluster) * 2 * p.cols;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const long long col = static_cast<long long>(j0 + k * q.team) * 8 - at.m;
-      if (!EDGE) {
-        if (mask[k]) {
-          store8(to + col, aw[k]);
-          store8(to + p.cols + col, ab[k]);
-        }
-      } else {
+      const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+      for (int h = 0; h < E / 4; ++h) {
+        if (mask[k] && !EDGE) {
+          *reinterpret_cast<uint4*>(to + col + 4 * h) = pack<float>(aw[k] + 2 * h);
+          *reinterpret_cast<uint4*>(to + p.cols + col + 4 * h) = pack<float>(ab[k] + 2 * h);
+        }
+      }
+      if (EDGE) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
           if ((mask[k] >> i) & 1u) {
-            to[col + i] = i & 1 ? aw[k][i / 2].y : aw[k][i / 2].x;
-            to[p.cols + col + i] = i & 1 ? ab[k][i / 2].y : ab[k][i / 2].x;
+            to[col + i] = element(aw[k], i);
+            to[p.cols + col + i] = element(ab[k], i);
           }
       }
     }
@@ -380,10 +418,10 @@ int column_parts(const mb_ln_desc* d) {
 }
 
 
-// Plan of the row kernel; two CTAs per SM where the registers allow.
+// Plan of the row kernel; one CTA per SM, so that there are few partial sums.
 bool plan_bwd(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
-  if (!plan_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, true, from_y, q)) return false;
-  size_grid(d->rows, q->per_thread == 1 ? 2 : 1, q);
+  if (!plan_bwd_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, from_y, q)) return false;
+  size_grid(d->rows, 1, q);
   return true;
 }
 
@@ -392,7 +430,7 @@ struct Grads { void *dw, *db; float* ws; };
 template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
 int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
   static std::atomic<int> cache[64];
-  auto kernel = ln_bwd_rows<T, K, FROM_Y, DSUM, DROP, EDGE, CLUSTER>;
+  auto kernel = ln_bwd_rows<T, K, bwd_rows_between_barriers(K), FROM_Y, DSUM, DROP, EDGE, CLUSTER>;
   int regs = 0;
   if (int rc = prepare("layer_norm_bwd", kernel, cache, &regs)) return rc;
   fit_clusters(kernel, &q);
@@ -403,14 +441,16 @@ int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
 
 template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
 int pick_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
-  if (q.cluster > 1) return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, true>(p, q, g, st);
+  constexpr int most = 16 / kE<T>;
+  if (q.cluster > 1) return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, true>(p, q, g, st);
   if (q.per_thread == 1) return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-  return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+  if (q.per_thread == 2) return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+  return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
 }
 
 template <typename T, bool FROM_Y, bool DSUM, bool DROP>
 int pick_edge(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
-  return p.cols % 8 ? pick_bwd<T, FROM_Y, DSUM, DROP, true>(p, q, g, st) : pick_bwd<T, FROM_Y, DSUM, DROP, false>(p, q, g, st);
+  return p.cols % kE<T> ? pick_bwd<T, FROM_Y, DSUM, DROP, true>(p, q, g, st) : pick_bwd<T, FROM_Y, DSUM, DROP, false>(p, q, g, st);
 }
 
 template <typename T, bool FROM_Y>
@@ -473,7 +513,8 @@ int mb_layer_norm_bwd(const void* dy, const void* kept, int kept_is_output, cons
   if ((dweight || dbias) && (!workspace || !aligned(workspace, 16) || workspace_bytes < mb_layer_norm_workspace_bytes(d)))
     return fail(MB_ERR_WORKSPACE, "%s: workspace too small or misaligned", who);
   const Grads g{dweight, dbias, static_cast<float*>(workspace)};
-  const bool granules = on_granules(d, {{dy, d->ld_a}, {kept, d->ld_b}, {dsum, d->ld_c}, {dv, d->cols}, {dx, d->cols}});
+  const bool granules = d->ld_a == d->cols && d->ld_b == d->cols && (!dsum || d->ld_c == d->cols) &&
+                        on_granules(d, {{dy, d->cols}, {kept, d->cols}, {dsum, d->cols}, {dv, d->cols}, {dx, d->cols}});
   auto go = [&](auto tag) {
     using T = decltype(tag);
     return kept_is_output ? bwd<T, true>(p, d, granules, g, st) : bwd<T, false>(p, d, granules, g, st);

@@ -4,193 +4,341 @@
 namespace mb {
 namespace {
 
-// Row statistics of `n` values: every warp centres on its own mean, and the warps' (count, mean,
-// squared deviations) are combined - no difference of large sums is ever formed.
-template <bool CLUSTER>
-__device__ __forceinline__ void combine_stats(WarpSums& red, float4 (*peer)[8], const RowPlan& q, const RowWalk& at, int buf,
-                                              float count, float& mean, float& m2, float n) {
-  const int warps = q.team >> 5, w0 = at.group * warps;
-  if ((threadIdx.x & 31) == 0) red.v[buf][threadIdx.x >> 5] = make_float4(count, mean, m2, 0.f);
-  team_barrier(at.group, q.team);
-  float s = 0.f, c = 0.f;
-  for (int i = 0; i < warps; ++i) {
-    const float4 f = red.v[buf][w0 + i];
-    s = fmaf(f.x, f.y, s);
-    c += f.x;
-  }
-  mean = c > 0.f ? s / c : 0.f;
-  m2 = 0.f;
-  for (int i = 0; i < warps; ++i) {
-    const float4 f = red.v[buf][w0 + i];
-    const float d = f.y - mean;
-    m2 += fmaf(f.x * d, d, f.z);
-  }
-  if (CLUSTER) {
-    if (threadIdx.x < q.cluster) put_remote(&peer[buf][at.rank], threadIdx.x, make_float4(c, mean, m2, 0.f));
-    cluster_barrier();
-    s = 0.f;
-    for (int i = 0; i < q.cluster; ++i) s = fmaf(peer[buf][i].x, peer[buf][i].y, s);
-    mean = s / n;
-    m2 = 0.f;
-    for (int i = 0; i < q.cluster; ++i) {
-      const float4 f = peer[buf][i];
-      const float d = f.y - mean;
-      m2 += fmaf(f.x * d, d, f.z);
-    }
-  }
+// ---- rows in registers -----------------------------------------------------------------------
+// Statistics: every warp centres on its own mean, and the warps' (count, sum, squared deviations)
+// are combined, so no difference of large sums is ever formed.  R rows share the shuffles and the
+// barrier of a reduction, which are what a row of a few hundred values waits for.
+
+// Residual add and dropout of a granule.
+template <typename T, int P>
+__device__ __forceinline__ void add_residual(const LnArgs& p, unsigned long long key, size_t granule, float2 (&v)[P], const float2 (&res)[P]) {
+  if (p.drop.on) apply_keep(v, keep_granule<T>(p.drop, key, granule), p.drop.scale);
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = add2(res[i], v[i]);
+}
+template <int P>
+__device__ __forceinline__ void normalise(float2 (&y)[P], float mean, float rstd, const float2 (&w)[P], const float2 (&b)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) y[i] = fma2(mul2(add2(y[i], both(-mean)), both(rstd)), w[i], b[i]);
+}
+template <int P>
+__device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, uint32_t mask, bool whole, float2 sum) {
+  float2 d[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) d[i] = add2(v[i], both(-mean));
+  if (!whole) zero_outside(d, mask);
+#pragma unroll
+  for (int i = 0; i < P; ++i) sum = fma2(d[i], d[i], sum);
+  return sum;
 }
 
-template <typename T, int K, bool RES, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxTeam) ln_fwd_rows(LnArgs p, RowPlan q) {
+template <typename T, int K, int R, bool RES, bool EDGE>
+__global__ void __launch_bounds__(kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
   extern __shared__ __align__(128) uint4 ring[];
-  if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
-  __shared__ WarpSums red;
-  __shared__ float4 peer[2][8];
-  constexpr int kOps = RES ? 2 : 1;
-  constexpr bool kKeep = K <= 2 && !CLUSTER;      // parameters of the thread's columns stay in registers
-  const RowWalk at(q, static_cast<int>(p.cols));
-  const int granules = EDGE ? static_cast<int>((at.m + p.cols + 7) >> 3) : static_cast<int>(p.cols >> 3);
-  const size_t total = p.rows * p.cols;
-  const float n = static_cast<float>(p.cols), inv_n = 1.f / n;
-  const unsigned long long key = p.drop.on ? __ldg(p.drop.seed) : 0;
+  __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
+  __shared__ float counts[kMaxThreads / 32];
+  constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1, kSlots = K * kOps;
+  constexpr int kParam = kParamUnits<T> * kUnit;
+  constexpr uint32_t kAll = (1u << E) - 1;
+  constexpr bool kInRegs = K == 1;
+  const RowWalk at(q, p.cols, E);
+  const float inv_n = 1.f / static_cast<float>(p.cols);
+  const int rows = static_cast<int>(p.rows), step = at.step, lane = threadIdx.x & 31, warps = q.team >> 5;
+  const unsigned long long key = RES && p.drop.on ? __ldg(p.drop.seed) : 0;
+  const uint32_t stride = (blockDim.x >> 5) * (kSlots * kUnit);
+  const uint32_t slots = sm100::smem_u32(ring) + (threadIdx.x >> 5) * (kSlots * kUnit) + lane * 16;
+  const uint32_t params = sm100::smem_u32(ring) + q.stages * stride + (at.t >> 5) * (K * 2 * kParam) + (at.t & 31) * 16;
+  const uint32_t kstep = q.team * 16;
 
-  long long col[K];
   uint32_t mask[K];
-  float wk[kKeep ? K : 1][8], bk[kKeep ? K : 1][8];
   float count = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int jl = at.t + k * q.team, j = at.rank * q.chunk + jl;
-    col[k] = static_cast<long long>(j) * 8 - at.m;
-    mask[k] = jl < q.chunk && j < granules ? 0xffu : 0u;
-    if (EDGE && mask[k]) {
-      if (col[k] < 0) mask[k] &= 0xffu << -col[k];
-      if (col[k] + 8 > static_cast<long long>(p.cols)) mask[k] &= 0xffu >> (col[k] + 8 - static_cast<long long>(p.cols));
-    }
+    mask[k] = column_mask<T, EDGE>(at, q, at.t + k * q.team, p.cols);
     count += static_cast<float>(__popc(mask[k]));
-    if (kKeep) {
-      param8<T>(p.w, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 1.f, wk[k]);
-      param8<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 0.f, bk[k]);
-    }
   }
-  const float warp_count = warp_sum(count);
+  if (!kInRegs) {
+    count = warp_sum(count);
+    if (lane == 0) counts[threadIdx.x >> 5] = count;
+  }
 
-  const int plane = q.chunk;                                   // granules per plane of one stage
-  const int per_op = plane * kPlanes<T>, per_stage = per_op * kOps;
-  uint4* mine = ring + static_cast<size_t>(at.group) * q.stages * per_stage + at.t;
-  const uint32_t mine_u = sm100::smem_u32(mine);
-
-  auto fetch = [&](size_t row, int stage) {
-    if (row < p.rows) {
+  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, at.t) * sizeof(T);
+  const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
+  // inputs may have gaps between their rows
+  size_t in_a = row_offset<T, EDGE>(at.first, p.ld_a, p.cols, at.t) * sizeof(T), in_b = RES ? row_offset<T, EDGE>(at.first, p.ld_b, p.cols, at.t) * sizeof(T) : 0;
+  int next = at.first;
+  auto fetch = [&](uint32_t stage) {
+    if (next < rows) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!mask[k]) continue;
-        const int j = at.rank * q.chunk + at.t + k * q.team;
-        const uint32_t dst = mine_u + (stage * per_stage + k * q.team) * 16;
-        if (EDGE) {
-          const size_t e = ((row * p.cols) >> 3) * 8 + static_cast<size_t>(j) * 8;
-          ring_fetch<T>(dst, plane, static_cast<const T*>(p.a) + e, total - e);
-          if (RES) ring_fetch<T>(dst + per_op * 16, plane, static_cast<const T*>(p.b) + e, total - e);
-        } else {
-          ring_fetch<T>(dst, plane, static_cast<const T*>(p.a) + row * p.ld_a + static_cast<size_t>(j) * 8);
-          if (RES) ring_fetch<T>(dst + per_op * 16, plane, static_cast<const T*>(p.b) + row * p.ld_b + static_cast<size_t>(j) * 8);
-        }
+        ring_copy<EDGE>(stage + (k * kOps) * kUnit, p.a, in_a + k * kstep, p.rows * p.cols * sizeof(T));
+        if (RES) ring_copy<EDGE>(stage + (k * kOps + 1) * kUnit, p.b, in_b + k * kstep, p.rows * p.cols * sizeof(T));
       }
+      in_a += static_cast<size_t>(step) * p.ld_a * sizeof(T);
+      if (RES) in_b += static_cast<size_t>(step) * p.ld_b * sizeof(T);
     }
-    cp_async_commit();
+    next += step;
   };
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (!mask[k])
+      for (int s = 0; s < q.stages; ++s)
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) smem_put(slots + s * stride + (k * kOps + o) * kUnit, make_uint4(0, 0, 0, 0));
+  for (int s = 0; s < q.stages; s += R) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) fetch(slots + (s + r) * stride);
+    cp_async_commit();
+  }
 
-  size_t ahead = at.first;
-  for (int s = 0; s < q.stages - 1; ++s, ahead += at.step) fetch(ahead, s);
-  // the teams of a warp shuffle together, so they leave the loop together
-  const size_t lead = q.team < 32 ? at.first - static_cast<size_t>(at.group - (threadIdx.x & ~31) / q.team) * q.period : at.first;
-  int stage = 0, fill = q.stages - 1, buf = 0;
-  size_t row = at.first;
-  for (size_t go = lead; go < p.rows; go += at.step, row += at.step, buf ^= 1) {
-    cp_async_wait(q.stages - 2);
-    float v[K][8];
-    float s = 0.f;
+  float2 wr[P], br[P];
+  if (kInRegs || at.group == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (mask[k] && row < p.rows) {
-        const uint4* src = mine + stage * per_stage + k * q.team;
-        ring_read<T>(src, plane, v[k]);
-        if (RES) {
-          float r[8];
-          ring_read<T>(src + per_op, plane, r);
-          uint32_t keep = 0xffu;
-          if (p.drop.on) {
-            const int j = at.rank * q.chunk + at.t + k * q.team;
-            keep = keep8(key, ((row * p.cols) >> 3) + j, p.drop.stream, p.drop.last);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            v[k][i] = __fadd_rn(r[i], !p.drop.on ? v[k][i] : (keep >> i) & 1u ? __fmul_rn(v[k][i], p.drop.scale) : 0.f);
-        }
-        if (EDGE && mask[k] != 0xffu) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[k][i] = (mask[k] >> i) & 1u ? v[k][i] : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[k][i];
-    }
-    fetch(ahead, fill);
-    ahead += at.step;
-    stage = stage + 1 == q.stages ? 0 : stage + 1;
-    fill = fill + 1 == q.stages ? 0 : fill + 1;
-
-    auto deviations = [&](float mean) {
-      float d2 = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float d = (EDGE ? (mask[k] >> i) & 1u : mask[k]) ? v[k][i] - mean : 0.f;
-          d2 = fmaf(d, d, d2);
-        }
-      return d2;
-    };
-    float mean, m2;
-    if (q.team <= 32) {
-      mean = lanes_sum(s, q.team) * inv_n;
-      m2 = lanes_sum(deviations(mean), q.team);
-    } else {
-      mean = warp_count > 0.f ? warp_sum(s) / warp_count : 0.f;
-      m2 = warp_sum(deviations(mean));
-      combine_stats<CLUSTER>(red, peer, q, at, buf, warp_count, mean, m2, n);
-    }
-    const float rstd = 1.f / sqrtf(m2 * inv_n + p.eps);
-    if (row < p.rows) {
-      if (at.t == 0 && at.rank == 0) {
-        p.mean[row] = mean;
-        p.rstd[row] = rstd;
-      }
-      const size_t base = EDGE ? ((row * p.cols) >> 3) * 8 : row * p.cols;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!mask[k]) continue;
-        const size_t e = base + static_cast<size_t>(at.rank * q.chunk + at.t + k * q.team) * 8;
-        if (p.out2) {
-          if (EDGE) store8_masked(static_cast<T*>(p.out2) + e, v[k], mask[k]);
-          else store8(static_cast<T*>(p.out2) + e, v[k]);
-        }
-        float w[8], b[8], y[8];
-        if (!kKeep) {
-          param8<T>(p.w, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 1.f, w);
-          param8<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col[k], mask[k], 0.f, b);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf((v[k][i] - mean) * rstd, kKeep ? wk[kKeep ? k : 0][i] : w[i], kKeep ? bk[kKeep ? k : 0][i] : b[i]);
-        if (EDGE) store8_masked(static_cast<T*>(p.out) + e, y, mask[k]);
-        else store8(static_cast<T*>(p.out) + e, y);
+      const long long col = static_cast<long long>(at.t + k * q.team) * E - at.m;
+      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, wr);
+      load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, br);
+      if (!kInRegs) {
+        param_put<T>(params + (2 * k) * kParam, wr);
+        param_put<T>(params + (2 * k + 1) * kParam, br);
       }
     }
   }
-  if (CLUSTER) cluster_barrier();      // no CTA leaves while a peer may still write into it
+  if (!kInRegs) __syncthreads();       // the parameters that group 0 put down, and the counts
+  // combining the warps' statistics, this lane looks after row lane % R of warp lane / R
+  const int part = lane / R;
+  const float part_count = q.team > 32 && part < warps ? counts[at.group * warps + part] : 0.f;
+  const float part_inv = part_count > 0.f ? 1.f / part_count : 0.f;
+
+  uint32_t stage = slots;
+  int row = at.first, buf = 0;
+  const int spare = at.spare(q);
+  for (; row - spare < rows; row += R * step, buf ^= 1) {
+    cp_async_wait(q.stages / R - 1);
+    float2 v[R][K][P];
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float2 sum = both(0.f);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        ring_get<T>(stage + r * stride + (k * kOps) * kUnit, v[r][k]);
+        if (RES) {
+          float2 res[P];
+          ring_get<T>(stage + r * stride + (k * kOps + 1) * kUnit, res);
+          add_residual<T>(p, key, (out + r * out_step + k * kstep) / 16, v[r][k], res);
+        }
+        if (EDGE && mask[k] != kAll) zero_outside(v[r][k], mask[k]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) sum = add2(sum, v[r][k][i]);
+      }
+      s[r] = sum.x + sum.y;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) fetch(stage + r * stride);       // the slots are free again
+    cp_async_commit();
+    stage += R * stride;
+    if (stage >= slots + q.stages * stride) stage = slots;
+
+    float mean[R], m2[R];
+    auto spread = [&](const float (&centre)[R], float (&d)[R]) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float2 sum = both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) sum = deviations(v[r][k], centre[r], mask[k], mask[k] == kAll, sum);
+        d[r] = sum.x + sum.y;
+      }
+    };
+    if (q.team <= 32) {
+      lanes_sums(s, q.team);
+#pragma unroll
+      for (int r = 0; r < R; ++r) mean[r] = s[r] * inv_n;
+      spread(mean, m2);
+      lanes_sums(m2, q.team);
+    } else {
+      const float x = warp_sums(s);
+#pragma unroll
+      for (int r = 0; r < R; ++r) mean[r] = count > 0.f ? __shfl_sync(0xffffffffu, x, r * (32 / R)) / count : 0.f;
+      spread(mean, m2);
+      const float y = warp_sums(m2);
+      if ((lane & (32 / R - 1)) == 0) red[buf][threadIdx.x >> 5][lane / (32 / R)] = make_float2(x, y);
+      team_barrier(at.group, q.team);
+      const float2 f = part < warps ? red[buf][at.group * warps + part][lane % R] : make_float2(0.f, 0.f);
+      float sum = f.x;
+#pragma unroll
+      for (int o = R; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      sum *= inv_n;
+      const float d = f.x * part_inv - sum;
+      float sq = part_count > 0.f ? fmaf(part_count * d, d, f.y) : 0.f;
+#pragma unroll
+      for (int o = R; o < 32; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        mean[r] = R == 1 ? sum : __shfl_sync(0xffffffffu, sum, r);
+        m2[r] = R == 1 ? sq : __shfl_sync(0xffffffffu, sq, r);
+      }
+    }
+    float rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      rstd[r] = 1.f / sqrtf(m2[r] * inv_n + p.eps);
+      if (at.t == 0 && row + r * step < rows) {
+        p.mean[row + r * step] = mean[r];
+        p.rstd[row + r * step] = rstd[r];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float2 w[P], b[P];
+      if constexpr (kInRegs) {
+        copy_pairs(wr, w);
+        copy_pairs(br, b);
+      } else {
+        param_get<T>(params + (2 * k) * kParam, w);
+        param_get<T>(params + (2 * k + 1) * kParam, b);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (!mask[k] || row + r * step >= rows) continue;
+        const size_t e = out + r * out_step + k * kstep;
+        if (RES && p.out2) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out2) + e), v[r][k], mask[k]);
+        normalise(v[r][k], mean[r], rstd[r], w, b);
+        store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), v[r][k], mask[k]);
+      }
+    }
+    out += R * out_step;
+  }
+}
+
+// ---- long rows ---------------------------------------------------------------------------------
+// A row lies in the shared memory of up to eight CTAs: it is read from HBM once and walked three
+// times there (sum, deviations, result).  Each granule's slot takes the next row's as soon as the
+// result is written, so that row arrives while this one is stored.
+template <typename T, bool RES, bool EDGE>
+__global__ void __launch_bounds__(kMaxTeam, 2) ln_fwd_long(LnArgs p, RowPlan q) {
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ float2 red[2][kMaxTeam / 32];
+  __shared__ float counts[kMaxTeam / 32];
+  __shared__ float peer[2][8][3];
+  constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1;
+  constexpr uint32_t kAll = (1u << E) - 1;
+  if (q.cluster > 1) cluster_barrier();      // every CTA has started before one writes into another
+  const RowWalk at(q, p.cols, E);
+  const float inv_n = 1.f / static_cast<float>(p.cols);
+  const int rows = static_cast<int>(p.rows), step = at.step, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned long long key = RES && p.drop.on ? __ldg(p.drop.seed) : 0;
+  const int j0 = at.rank * q.chunk + at.t;
+  const uint32_t slots = sm100::smem_u32(ring) + warp * (q.per_thread * kOps * kUnit) + lane * 16;
+  constexpr uint32_t kStep = kMaxTeam * 16;
+
+  auto mask_of = [&](int k) { return column_mask<T, EDGE>(at, q, at.t + k * kMaxTeam, p.cols); };
+  const int mine = at.t < q.chunk ? (q.chunk - at.t + kMaxTeam - 1) / kMaxTeam : 0;      // granules of this thread, some perhaps empty
+  float count = 0.f;
+  for (int k = 0; k < mine; ++k) count += static_cast<float>(__popc(mask_of(k)));
+  count = warp_sum(count);
+  if (lane == 0) counts[warp] = count;
+
+  auto fetch = [&](int row, int k) {
+    if (row >= rows || !mask_of(k)) return;
+    const size_t a = row_offset<T, EDGE>(row, p.ld_a, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
+    ring_copy<EDGE>(slots + (k * kOps) * kUnit, p.a, a, p.rows * p.cols * sizeof(T));
+    if (RES) {
+      const size_t b = row_offset<T, EDGE>(row, p.ld_b, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
+      ring_copy<EDGE>(slots + (k * kOps + 1) * kUnit, p.b, b, p.rows * p.cols * sizeof(T));
+    }
+  };
+  // with a residual the sum is kept as fp32 in the granule's two slots
+  auto value = [&](int k, float2 (&v)[P]) {
+    if constexpr (RES) param_get<T>(slots + (k * kOps) * kUnit, v);
+    else ring_get<T>(slots + (k * kOps) * kUnit, v);
+  };
+
+  for (int k = 0; k < mine; ++k) fetch(at.first, k);
+  cp_async_commit();
+  __syncthreads();
+  int buf = 0;
+  for (int row = at.first; row < rows; row += step, buf ^= 1) {
+    const size_t out = row_offset<T, EDGE>(row, p.cols, p.cols, j0) * sizeof(T);
+    cp_async_wait(0);
+    float2 sum = both(0.f);
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k) {
+      const uint32_t m = mask_of(k);
+      if (!m) continue;
+      float2 v[P];
+      ring_get<T>(slots + (k * kOps) * kUnit, v);
+      if (RES) {
+        float2 res[P];
+        ring_get<T>(slots + (k * kOps + 1) * kUnit, res);
+        add_residual<T>(p, key, (out + static_cast<size_t>(k) * kStep) / 16, v, res);
+        param_put<T>(slots + (k * kOps) * kUnit, v);
+      }
+      if (EDGE && m != kAll) zero_outside(v, m);
+#pragma unroll
+      for (int i = 0; i < P; ++i) sum = add2(sum, v[i]);
+    }
+    const float x = warp_sum(sum.x + sum.y), centre = count > 0.f ? x / count : 0.f;
+    float2 dev = both(0.f);
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k) {
+      const uint32_t m = mask_of(k);
+      if (!m) continue;
+      float2 v[P];
+      value(k, v);
+      dev = deviations(v, centre, m, !EDGE || m == kAll, dev);
+    }
+    const float y = warp_sum(dev.x + dev.y);
+    if (lane == 0) red[buf][warp] = make_float2(x, y);
+    __syncthreads();
+    float mean, m2;
+    {
+      constexpr int kWarps = kMaxTeam / 32;
+      const float2 f = lane < kWarps ? red[buf][lane] : make_float2(0.f, 0.f);
+      const float c = lane < kWarps ? counts[lane] : 0.f;
+      const float total = warp_sum(f.x), n = warp_sum(c);
+      const float m = n > 0.f ? total / n : 0.f;
+      const float d = c > 0.f ? f.x / c - m : 0.f;
+      m2 = warp_sum(fmaf(c * d, d, f.y));
+      mean = m;
+      if (q.cluster > 1) {
+        if (threadIdx.x < q.cluster) {
+          put_remote(&peer[buf][at.rank][0], threadIdx.x, total);
+          put_remote(&peer[buf][at.rank][1], threadIdx.x, m2);
+          put_remote(&peer[buf][at.rank][2], threadIdx.x, n);
+        }
+        cluster_barrier();
+        const bool have = lane < q.cluster;
+        const float ps = have ? peer[buf][lane][0] : 0.f, pq = have ? peer[buf][lane][1] : 0.f, pn = have ? peer[buf][lane][2] : 0.f;
+        mean = warp_sum(ps) * inv_n;
+        const float pd = pn > 0.f ? ps / pn - mean : 0.f;
+        m2 = warp_sum(fmaf(pn * pd, pd, pq));
+      }
+    }
+    const float rstd = 1.f / sqrtf(m2 * inv_n + p.eps);
+    if (threadIdx.x == 0 && at.rank == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k) {
+      const uint32_t m = mask_of(k);
+      if (!m) continue;
+      const long long col = static_cast<long long>(j0 + k * kMaxTeam) * E - at.m;
+      float2 v[P], w[P], b[P];
+      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, m, 1.f, w);
+      load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, m, 0.f, b);
+      value(k, v);
+      const size_t e = out + static_cast<size_t>(k) * kStep;
+      if (RES && p.out2) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out2) + e), v, m);
+      normalise(v, mean, rstd, w, b);
+      store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), v, m);
+      fetch(row + step, k);
+    }
+    cp_async_commit();
+  }
+  if (q.cluster > 1) cluster_barrier();      // no CTA leaves while a peer may still write into it
 }
 
 template <typename T>
@@ -231,10 +379,8 @@ __global__ void __launch_bounds__(kBlock) ln_fwd_any(LnArgs p) {
 }
 
 
-template <typename T, int K, bool RES, bool EDGE, bool CLUSTER>
-int launch_fwd(const LnArgs& p, RowPlan q, cudaStream_t st) {
-  static std::atomic<int> cache[64];
-  auto kernel = ln_fwd_rows<T, K, RES, EDGE, CLUSTER>;
+template <typename Kernel>
+int launch_fwd(Kernel kernel, std::atomic<int>* cache, const LnArgs& p, RowPlan q, cudaStream_t st) {
   int regs = 0;
   if (int rc = prepare("layer_norm_fwd", kernel, cache, &regs)) return rc;
   size_grid(p.rows, resident(q.groups * q.team, regs, q.smem), &q);
@@ -242,21 +388,40 @@ int launch_fwd(const LnArgs& p, RowPlan q, cudaStream_t st) {
   return launch_rows("layer_norm_fwd", kernel, q, st, p, q);
 }
 
+template <typename T, int K, bool RES, bool EDGE>
+int rows_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
+  static std::atomic<int> cache[64];
+  return launch_fwd(ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE>, cache, p, q, st);
+}
+
+template <typename T, bool RES, bool EDGE>
+int long_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
+  static std::atomic<int> cache[64];
+  return launch_fwd(ln_fwd_long<T, RES, EDGE>, cache, p, q, st);
+}
+
 template <typename T, bool RES, bool EDGE>
 int pick_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
-  if (q.cluster > 1) return q.per_thread <= 4 ? launch_fwd<T, 4, RES, EDGE, true>(p, q, st) : launch_fwd<T, 8, RES, EDGE, true>(p, q, st);
-  if (q.per_thread == 1) return launch_fwd<T, 1, RES, EDGE, false>(p, q, st);
-  if (q.per_thread == 2) return launch_fwd<T, 2, RES, EDGE, false>(p, q, st);
-  return launch_fwd<T, 4, RES, EDGE, false>(p, q, st);
+  switch (q.per_thread) {
+    case 1: return rows_fwd<T, 1, RES, EDGE>(p, q, st);
+    case 2: return rows_fwd<T, 2, RES, EDGE>(p, q, st);
+    case 4: return rows_fwd<T, 4, RES, EDGE>(p, q, st);
+    default: return rows_fwd<T, 32 / kE<T>, RES, EDGE>(p, q, st);
+  }
 }
 
 template <typename T>
 int fwd(const LnArgs& p, bool granules, cudaStream_t st) {
   RowPlan q;
-  if (granules && plan_rows(p.rows, p.cols, sizeof(T), p.b ? 2 : 1, false, false, &q)) {
-    const bool edge = p.cols % 8 != 0;
+  const int ops = p.b ? 2 : 1;
+  const bool edge = p.cols % kE<T> != 0;
+  if (granules && plan_fwd_rows(p.rows, p.cols, sizeof(T), ops, &q)) {
     if (p.b) return edge ? pick_fwd<T, true, true>(p, q, st) : pick_fwd<T, true, false>(p, q, st);
     return edge ? pick_fwd<T, false, true>(p, q, st) : pick_fwd<T, false, false>(p, q, st);
+  }
+  if (granules && plan_fwd_long(p.rows, p.cols, sizeof(T), ops, &q)) {
+    if (p.b) return edge ? long_fwd<T, true, true>(p, q, st) : long_fwd<T, true, false>(p, q, st);
+    return edge ? long_fwd<T, false, true>(p, q, st) : long_fwd<T, false, false>(p, q, st);
   }
   ln_fwd_any<T><<<grid_for(p.rows, 1, 8), kBlock, 0, st>>>(p);
   return after_launch("layer_norm_fwd");
