@@ -1,5 +1,7 @@
 // Dropout from the counter-based generator (philox.cuh).  The backward is the same map applied to
-// the gradient.  Bound by HBM: it reads and writes each element once.
+// the gradient.  Bound by HBM: it reads and writes each element once; the generator's ten rounds per
+// eight elements stay below that.
+#include <type_traits>
 #include "philox.cuh"
 #include "types.cuh"
 
@@ -10,21 +12,99 @@ constexpr int kBlock = 256;
 
 // One thread per block of eight elements; any alignment.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) dropout_any(const T* x, T* y, size_t n, Drop d) {
-  const unsigned long long key = d.on ? __ldg(d.seed) : 0;
-  const size_t blocks = (n + 7) / 8;
-  for (size_t b = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; b < blocks; b += static_cast<size_t>(gridDim.x) * kBlock) {
-    const uint32_t keep = d.on ? keep8(key, b, d.stream, d.last) : 0xffu;
-    const size_t i0 = b * 8;
-    const int m = n - i0 < 8 ? static_cast<int>(n - i0) : 8;
-    for (int j = 0; j < m; ++j) y[i0 + j] = from_f32<T>((keep >> j) & 1u ? to_f32(x[i0 + j]) * d.scale : 0.f);
+__device__ __forceinline__ void drop_block(const T* x, T* y, size_t n, size_t b, const Drop& d, unsigned long long key) {
+  const unsigned long long one[1] = {b};
+  Dropped f[1] = {};
+  if (d.on) dropped<1>(d, key, one, f);
+  const uint32_t all = fold(f[0]);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const size_t i = b * 8 + j;
+    if (i < n) y[i] = from_f32<T>(unfold(all, j >> 1) & (j & 1 ? 0x80000000u : 0x8000u) ? 0.f : to_f32(x[i]) * d.scale);
   }
 }
 
 template <typename T>
+__global__ void __launch_bounds__(kBlock) dropout_any(const T* x, T* y, size_t n, Drop d) {
+  const unsigned long long key = d.on ? __ldg(d.seed) : 0;
+  const size_t blocks = (n + 7) / 8;
+  for (size_t b = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x; b < blocks; b += static_cast<size_t>(gridDim.x) * kBlock)
+    drop_block(x, y, n, b, d, key);
+}
+
+// Eight elements as one access: 16 bytes of a 16-bit type, 32 of fp32.
+template <typename T> struct Eight {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
+  __device__ __forceinline__ void drop(const Dropped& f, float scale) {
+    uint32_t* w = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        const __half2 h = __floats2half2_rn(a.x * scale, a.y * scale);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(w[i] << 16) * scale, __uint_as_float(w[i] & 0xffff0000u) * scale);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      w[i] &= ~sign_halves(f.d[i]);
+    }
+  }
+};
+template <> struct Eight<float> {
+  f8 v;
+  __device__ __forceinline__ void load(const float* p) { v = ld8(p); }
+  __device__ __forceinline__ void store(float* p) const { st8(p, v); }
+  __device__ __forceinline__ void drop(const Dropped& f, float scale) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v.v[2 * i] = zero_if(v.v[2 * i] * scale, sign_low(f.d[i]));
+      v.v[2 * i + 1] = zero_if(v.v[2 * i + 1] * scale, sign_high(f.d[i]));
+    }
+  }
+};
+
+// x and y aligned to eight elements.  A thread has AHEAD blocks in flight.
+template <typename T, int AHEAD>
+__global__ void __launch_bounds__(kBlock) dropout_eights(const T* x, T* y, size_t n, Drop d) {
+  const unsigned long long key = d.on ? __ldg(d.seed) : 0;
+  const size_t blocks = n / 8, first = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x, step = static_cast<size_t>(gridDim.x) * kBlock;
+  for (size_t b = first; b < blocks; b += AHEAD * step) {
+    Eight<T> e[AHEAD];
+    unsigned long long at[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      at[u] = b + u * step;
+      if (at[u] < blocks) e[u].load(x + at[u] * 8);
+    }
+    Dropped f[AHEAD] = {};
+    if (d.on) dropped<AHEAD>(d, key, at, f);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (at[u] >= blocks) break;
+      e[u].drop(f[u], d.scale);
+      e[u].store(y + at[u] * 8);
+    }
+  }
+  if (first == 0 && n % 8) drop_block(x, y, n, blocks, d, key);
+}
+
+template <typename T>
 int run(const void* x, void* y, size_t n, const Drop& d, cudaStream_t st) {
-  const int grid = grid_for((n + 7) / 8, kBlock, 8);
-  dropout_any<T><<<grid, kBlock, 0, st>>>(static_cast<const T*>(x), static_cast<T*>(y), n, d);
+  const T* from = static_cast<const T*>(x);
+  T* to = static_cast<T*>(y);
+  const size_t blocks = (n + 7) / 8;
+  const int grid = grid_for(blocks, kBlock, 8);
+  if (!aligned(x, 8 * sizeof(T)) || !aligned(y, 8 * sizeof(T)))
+    dropout_any<T><<<grid, kBlock, 0, st>>>(from, to, n, d);
+  // As many blocks as threads: more in flight would only be generated for nothing (176 x 4096 fp32:
+  // 6.9 us with 4, 4.4 with 1; 67 million bf16 values: 61 us with 1, 48 with 4).
+  else if (blocks <= static_cast<size_t>(grid) * kBlock)
+    dropout_eights<T, 1><<<grid, kBlock, 0, st>>>(from, to, n, d);
+  else
+    dropout_eights<T, 8 / static_cast<int>(sizeof(T))><<<grid, kBlock, 0, st>>>(from, to, n, d);
   return after_launch("dropout");
 }
 

@@ -46,16 +46,16 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-// Rows whose tensors lie on granule boundaries in the same way are walked in granules (rows.cuh), one
-// thread holding up to 16 values (32 forward, where there are no column sums) and a team up to
-// kMaxTeam threads.  Longer rows: forward stays in the shared memory of up to eight CTAs, backward in
-// the registers of up to eight.  Everything else takes the element-wise kernels.
-constexpr size_t kSmemLimit = 216 * 1024;
+// Rows whose tensors lie on granule boundaries in the same way are walked in granules (rows.cuh): a
+// thread holds 4 to 32 values, a team up to kMaxTeam threads.  Longer rows: forward stays in the shared
+// memory of up to eight CTAs, backward in the registers of up to eight.  Everything else takes the
+// element-wise kernels.
+constexpr size_t kSmemLimit = 225 * 1024;
 
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 // Rows between two barriers of the backward kernel with k granules a thread.
 constexpr int bwd_rows_between_barriers(int k) { return k == 1 ? 2 : 1; }
-constexpr int fwd_rows_between_barriers(int k, int elems) { return k * elems <= 16 ? 2 : 1; }
+constexpr int fwd_rows_between_barriers(int k, int elems) { return k == 1 ? 2 : 1; }
 
 // The period of the rows' alignment, and the granules that a row can touch.
 inline size_t row_granules(size_t cols, int elems, int* period) {
@@ -65,52 +65,84 @@ inline size_t row_granules(size_t cols, int elems, int* period) {
   return (cols + (elems - g) + elems - 1) / elems;
 }
 
-// Threads for `chunk` granules of up to `most` a thread; false if they do not fit a team.
-inline bool plan_team(int chunk, int most, RowPlan* q) {
+// A team for `chunk` granules with `values` values a thread.
+inline void plan_team(int chunk, int elems, int values, RowPlan* q) {
   q->chunk = chunk;
-  q->per_thread = 1;
   if (chunk <= 32) {                   // several rows a warp, or one
+    q->per_thread = 1;
     for (q->team = 1; q->team < chunk;) q->team *= 2;
-    return true;
+    return;
   }
-  while (q->per_thread < most && chunk > 32 * q->per_thread) q->per_thread *= 2;    // one warp if possible: no barrier
+  q->per_thread = values / elems;
   q->team = ceil_div(chunk, 32 * q->per_thread) * 32;
-  return q->team <= kMaxTeam;
 }
+// Rows of up to 1024 values take one warp each, which needs no barrier: the fewest values a thread
+// then, or 0.  (30000 x 1001 bf16 backward: 46 us against 60 with two warps a row.)  The choice goes by
+// the length of a row alone, not by the number of rows, so that a row's result does not depend on how
+// many others there are; a few rows are served a little slower for it (2051 x 1000 fp32, fused forward
+// and backward: 39 us against 34 with two warps).
+inline int one_warp_values(int chunk, int elems) {
+  int v = 2 * elems;
+  while (v < 32 && chunk * elems > 32 * v) v *= 2;
+  return chunk * elems <= 32 * v ? v : 0;
+}
+inline int cta_threads(const RowPlan& q, int elems) { return q.per_thread * elems >= 32 ? kMaxThreadsWide : kMaxThreads; }
 
-// Teams per CTA: as many as `threads` hold, fewer where the rows would not reach every SM.
-inline void plan_groups(size_t rows, int threads, RowPlan* q) {
-  q->groups = q->cluster > 1 ? 1 : threads / q->team;
+// Teams per CTA: at most `most`, or as few as give no team more rows than that would.
+inline void plan_groups(size_t rows, int most, RowPlan* q) {
+  q->groups = q->cluster > 1 || most < 1 ? 1 : most;
   if (q->team > 32 && q->groups > 15) q->groups = 15;        // named barriers
-  const size_t spread = (rows + num_sms() - 1) / num_sms();
-  if (static_cast<size_t>(q->groups) > spread) q->groups = static_cast<int>(spread);
+  const size_t sms = num_sms(), each = (rows + sms * q->groups - 1) / (sms * q->groups);
+  q->groups = static_cast<int>((rows + sms * each - 1) / (sms * each));
   if (q->groups < 1) q->groups = 1;
   if (q->team < 32) q->groups = (q->groups + 32 / q->team - 1) / (32 / q->team) * (32 / q->team);    // whole warps
+}
+
+// The ring beside `params` bytes: as many rows ahead as fit, up to eight; false if not even `least`
+// times the r rows between two barriers do.
+inline bool plan_ring(int r, int ops, int least, size_t params, RowPlan* q) {
+  const size_t stage = static_cast<size_t>(ceil_div(q->groups * q->team, 32)) * q->per_thread * ops * kUnit;
+  if (params >= kSmemLimit) return false;
+  const size_t deep = (kSmemLimit - params) / (r * stage);
+  if (deep < static_cast<size_t>(least)) return false;
+  q->stages = r * static_cast<int>(deep > static_cast<size_t>(8 / r) ? 8 / r : deep);
+  q->smem = stage * q->stages + params;
+  return true;
 }
 
 inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from_y, RowPlan* q) {
   if (rows >> 30) return false;                              // row numbers are 32-bit, and some steps ahead
   const int elems = 16 / elem;
   const size_t most = row_granules(cols, elems, &q->period);
-  if (most > static_cast<size_t>(kMaxTeam) * 8 * (16 / elems)) return false;
+  if (most > static_cast<size_t>(kMaxTeam) * 8 * (32 / elems)) return false;
   for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
-    if (!plan_team(ceil_div(most, q->cluster), 16 / elems, q)) continue;
-    if (q->cluster > 1) {                                    // the cluster's kernel has 16 values a thread
-      q->per_thread = 16 / elems;
-      q->team = ceil_div(q->chunk, 32 * q->per_thread) * 32;
+    const int chunk = ceil_div(static_cast<long long>(most), q->cluster);
+    // the fp32 weight (with from_y also minus the bias) lies beside the ring
+    const size_t params_row = static_cast<size_t>(chunk) * elems * 4 * (from_y ? 2 : 1), row = static_cast<size_t>(chunk) * 16 * ops;
+    const size_t deep = params_row < kSmemLimit ? (kSmemLimit - params_row) / row : 0;
+    // What bounds these kernels is the bytes on their way: three rows a team where shared memory holds
+    // six, so one is at work and two arrive, and as many values a thread as leave the CTA 512 threads
+    // (fp32 8192 x 4096 with dsum: 129 us with one team of 512, 166 with two of 256; bf16 16384 x 4096:
+    // 70 us with four teams of 128, 74 with three of 256).
+    int teams = deep >= 6 ? static_cast<int>(deep / 3) : deep >= 5 ? 2 : 1, values = q->cluster > 1 ? 32 : one_warp_values(chunk, elems);
+    if (!values) {
+      values = 32;
+      while (values > 8 && values > 2 * elems && static_cast<long long>(chunk) * elems / values * teams < 512 &&
+             static_cast<long long>(chunk) * elems * 2 / values <= kMaxTeam)
+        values /= 2;
     }
-    plan_groups(rows, kMaxThreads, q);
-    // one CTA per SM; the fp32 weight (with from_y its inverse and the bias) beside the ring
-    const int r = bwd_rows_between_barriers(q->per_thread);
-    const size_t stage = static_cast<size_t>(q->groups * q->team / 32) * q->per_thread * ops * kUnit;
-    const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 4 * (from_y ? 3 : 1);
-    const size_t deep = (kSmemLimit - params) / (r * stage);
-    if (deep < 2) continue;
-    q->stages = r * static_cast<int>(deep > 8 / r ? 8 / r : deep);
-    q->smem = stage * q->stages + params;
-    const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
-    if (fold > q->smem) q->smem = fold;                      // the teams' column sums are folded there
-    return q->smem <= kSmemLimit;
+    plan_team(chunk, elems, values, q);
+    if (q->team > kMaxTeam) continue;
+    const int r = bwd_rows_between_barriers(q->per_thread), fit = cta_threads(*q, elems) / q->team;
+    const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 4 * (from_y ? 2 : 1);
+    for (teams = q->team <= 32 || teams > fit ? fit : teams; teams >= 1; --teams) {
+      plan_groups(rows, teams, q);
+      const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
+      if (fold <= kSmemLimit && plan_ring(r, ops, 2, params, q)) {
+        if (fold > q->smem) q->smem = fold;                  // the teams' column sums are folded there
+        return true;
+      }
+    }
   }
   return false;
 }
@@ -121,20 +153,18 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   const size_t most = row_granules(cols, elems, &q->period);
   q->cluster = 1;
   if (most > static_cast<size_t>(kMaxTeam) * (32 / elems)) return false;
-  if (!plan_team(static_cast<int>(most), 16 / elems, q)) {
-    q->per_thread = 32 / elems;
-    q->team = ceil_div(static_cast<int>(most), 32 * q->per_thread) * 32;
-  }
-  plan_groups(rows, kMaxThreads, q);
+  const int chunk = static_cast<int>(most);
+  int values = one_warp_values(chunk, elems);
+  if (!values) values = 32;      // (16384 x 8192 bf16: 115 us against 154 with 16)
+  plan_team(chunk, elems, values, q);
+  if (q->team > kMaxTeam) return false;
   const int r = fwd_rows_between_barriers(q->per_thread, elems);
-  const size_t stage = static_cast<size_t>(q->groups * q->team / 32) * q->per_thread * ops * kUnit;
   const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
-  const size_t budget = (q->groups * q->team > kMaxThreads / 2 ? kSmemLimit : 100 * 1024) - params;
-  const size_t deep = budget / (r * stage);
-  if (deep < 1) return false;
-  q->stages = r * static_cast<int>(deep > 8 / r ? 8 / r : deep);
-  q->smem = stage * q->stages + params;
-  return true;
+  for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
+    plan_groups(rows, teams, q);
+    if (plan_ring(r, ops, teams == 1 ? 1 : 2, params, q)) return true;
+  }
+  return false;
 }
 
 // One row in the shared memory of 1 to 8 CTAs, of which two share an SM if they are small enough.

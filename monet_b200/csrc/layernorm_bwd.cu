@@ -15,12 +15,12 @@ namespace {
 // With t = v - mean or y - b:  sum g xhat = rstd sum (dy t) w  or  sum dy t  (the weight cancels), and
 // dw = sum over rows of (dy t) rstd  or  (sum dy t) / w, so xhat itself is never formed.
 template <typename T, int K, int R, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
+__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float red[2][kMaxThreads / 32][2 * R];      // double-buffered by row: one barrier a row
   __shared__ float peer[2][8][2 * R];
   if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
-  constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 3 : 1;
+  constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 2 : 1;
   constexpr int kParam = kParamUnits<T> * kUnit;
   constexpr bool kInRegs = K == 1;
   const RowWalk at(q, p.cols, E);
@@ -52,15 +52,12 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
         if (mask[k]) ring_copy<EDGE>(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, p.rows * p.cols * sizeof(T));
   };
 
-  float2 wr[P], nbr[P], iwr[P];        // kInRegs: the weight; with FROM_Y minus the bias and 1 / weight
+  float2 wr[P], nbr[P];                // kInRegs: the weight; with FROM_Y minus the bias
   auto weight = [&](int k, float2 v[P]) {
     if constexpr (kInRegs) copy_pairs(wr, v); else param_get<T>(params + (k * kKinds) * kParam, v);
   };
   auto minus_bias = [&](int k, float2 v[P]) {
     if constexpr (kInRegs) copy_pairs(nbr, v); else param_get<T>(params + (k * kKinds + 1) * kParam, v);
-  };
-  auto inverse_weight = [&](int k, float2 v[P]) {
-    if constexpr (kInRegs) copy_pairs(iwr, v); else param_get<T>(params + (k * kKinds + 2) * kParam, v);
   };
   // t and dy of one granule; zero outside the row
   auto read = [&](uint32_t stage, int k, float mean, float2 (&t)[P], float2 (&dy)[P]) {
@@ -96,9 +93,6 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
       load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, v);
       if constexpr (kInRegs) copy_pairs(v, wr); else param_put<T>(params + (k * kKinds) * kParam, v);
       if (FROM_Y) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) v[i] = make_float2(1.f / v[i].x, 1.f / v[i].y);
-        if constexpr (kInRegs) copy_pairs(v, iwr); else param_put<T>(params + (k * kKinds + 2) * kParam, v);
         load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, v);
 #pragma unroll
         for (int i = 0; i < P; ++i) v[i] = make_float2(-v[i].x, -v[i].y);
@@ -174,14 +168,22 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
         gather(peer[buf][0], q.cluster, s);
       }
     }
-    uint32_t keep[K];
+    uint32_t gone[R][K];                 // what dropout drops, the pairs' sign bits folded into a word
     if (DROP) {
       const unsigned long long key = __ldg(p.drop.seed);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        keep[k] = 0;
-#pragma unroll 1
-        for (int r = R - 1; r >= 0; --r) keep[k] = keep[k] << E | keep_granule<T>(p.drop, key, (out + r * out_step + k * kstep) / 16);
+      for (int r = 0; r < R; ++r) {
+        size_t g[K];
+        Signs<T> s8[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) g[k] = (out + r * out_step + k * kstep) / 16;
+        granule_signs<T, K>(p.drop, key, g, s8);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          gone[r][k] = 0;
+#pragma unroll
+          for (int i = 0; i < P; ++i) gone[r][k] |= (s8[k].d[i] & 0x80008000u) >> i;
+        }
       }
     }
 #pragma unroll
@@ -198,10 +200,8 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
 #pragma unroll
         for (int i = 0; i < P; ++i) d[i] = fma2(d[i], w[i], c1);
         if (FROM_Y) {
-          float2 iw[P];
-          inverse_weight(k, iw);
 #pragma unroll
-          for (int i = 0; i < P; ++i) t[i] = mul2(t[i], iw[i]);
+          for (int i = 0; i < P; ++i) t[i] = mul2(t[i], make_float2(reciprocal(w[i].x), reciprocal(w[i].y)));
         }
 #pragma unroll
         for (int i = 0; i < P; ++i) d[i] = fma2(t[i], c2, d[i]);
@@ -216,7 +216,10 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
         const size_t e = out + r * out_step + k * kstep;
         if (mask[k]) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), d, mask[k]);
         if (DROP) {
-          apply_keep(d, keep[k] >> (E * r), p.drop.scale);
+          Signs<T> s8;
+#pragma unroll
+          for (int i = 0; i < P; ++i) s8.d[i] = gone[r][k] << i;
+          apply_signs<T>(d, s8, p.drop.scale);
           if (mask[k]) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out2) + e), d, mask[k]);
         }
       }
@@ -240,10 +243,10 @@ __global__ void __launch_bounds__(kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, 
   if (FROM_Y) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float2 iw[P];
-      inverse_weight(k, iw);
+      float2 w[P];
+      weight(k, w);
 #pragma unroll
-      for (int i = 0; i < P; ++i) aw[k][i] = mul2(aw[k][i], iw[i]);
+      for (int i = 0; i < P; ++i) aw[k][i] = make_float2(aw[k][i].x / w[i].x, aw[k][i].y / w[i].y);
     }
   }
   // the CTA's teams hold the same columns: halve their number until one is left
@@ -441,11 +444,14 @@ int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
 
 template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
 int pick_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
-  constexpr int most = 16 / kE<T>;
+  constexpr int most = 32 / kE<T>;
   if (q.cluster > 1) return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, true>(p, q, g, st);
-  if (q.per_thread == 1) return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-  if (q.per_thread == 2) return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-  return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+  switch (q.per_thread) {
+    case 1: return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+    case 2: return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+    case 4: return launch_bwd<T, 4, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+    default: return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+  }
 }
 
 template <typename T, bool FROM_Y, bool DSUM, bool DROP>

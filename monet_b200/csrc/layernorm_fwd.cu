@@ -9,13 +9,6 @@ namespace {
 // are combined, so no difference of large sums is ever formed.  R rows share the shuffles and the
 // barrier of a reduction, which are what a row of a few hundred values waits for.
 
-// Residual add and dropout of a granule.
-template <typename T, int P>
-__device__ __forceinline__ void add_residual(const LnArgs& p, unsigned long long key, size_t granule, float2 (&v)[P], const float2 (&res)[P]) {
-  if (p.drop.on) apply_keep(v, keep_granule<T>(p.drop, key, granule), p.drop.scale);
-#pragma unroll
-  for (int i = 0; i < P; ++i) v[i] = add2(res[i], v[i]);
-}
 template <int P>
 __device__ __forceinline__ void normalise(float2 (&y)[P], float mean, float rstd, const float2 (&w)[P], const float2 (&b)[P]) {
 #pragma unroll
@@ -33,7 +26,7 @@ __device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, u
 }
 
 template <typename T, int K, int R, bool RES, bool EDGE>
-__global__ void __launch_bounds__(kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
+__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
   __shared__ float counts[kMaxThreads / 32];
@@ -121,13 +114,22 @@ __global__ void __launch_bounds__(kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) 
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float2 sum = both(0.f);
+      Signs<T> gone[K];
+      if (RES && p.drop.on) {
+        size_t g[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k) g[k] = (out + r * out_step + k * kstep) / 16;
+        granule_signs<T, K>(p.drop, key, g, gone);
+      }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         ring_get<T>(stage + r * stride + (k * kOps) * kUnit, v[r][k]);
         if (RES) {
           float2 res[P];
+          if (p.drop.on) apply_signs<T>(v[r][k], gone[k], p.drop.scale);
           ring_get<T>(stage + r * stride + (k * kOps + 1) * kUnit, res);
-          add_residual<T>(p, key, (out + r * out_step + k * kstep) / 16, v[r][k], res);
+#pragma unroll
+          for (int i = 0; i < P; ++i) v[r][k][i] = add2(res[i], v[r][k][i]);
         }
         if (EDGE && mask[k] != kAll) zero_outside(v[r][k], mask[k]);
 #pragma unroll
@@ -272,7 +274,14 @@ __global__ void __launch_bounds__(kMaxTeam, 2) ln_fwd_long(LnArgs p, RowPlan q) 
       if (RES) {
         float2 res[P];
         ring_get<T>(slots + (k * kOps + 1) * kUnit, res);
-        add_residual<T>(p, key, (out + static_cast<size_t>(k) * kStep) / 16, v, res);
+        if (p.drop.on) {
+          const size_t g[1] = {(out + static_cast<size_t>(k) * kStep) / 16};
+          Signs<T> gone[1];
+          granule_signs<T, 1>(p.drop, key, g, gone);
+          apply_signs<T>(v, gone[0], p.drop.scale);
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[i] = add2(res[i], v[i]);
         param_put<T>(slots + (k * kOps) * kUnit, v);
       }
       if (EDGE && m != kAll) zero_outside(v, m);

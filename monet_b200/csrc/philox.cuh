@@ -5,9 +5,9 @@
 // numbers: as easy as 1, 2, 3", SC 2011) keyed by the 64-bit seed turns the counter (block low,
 // block high, stream, h) into four words = eight 16-bit halves, low half first.  Half i % 8 of
 // h = 0 is the upper half of the element's 32-bit number u, that of h = 1 the lower half.  The
-// element is dropped when u < round(p 2^32).  Comparing the upper halves decides all but one
-// element in 65536, so the second evaluation (h = 1) runs on a tie only: the cost is ten rounds
-// per eight elements, the resolution of p is 2^-32.
+// element is dropped when u < round(p 2^32).  The upper halves decide nearly always, so the second
+// evaluation (h = 1) runs on a tie only: the cost is ten rounds per eight elements, the resolution
+// of p is 2^-32.
 #pragma once
 #include "common.cuh"
 
@@ -37,58 +37,103 @@ inline int make_drop(const char* who, const mb_dropout_desc* d, Drop* out) {
   return MB_OK;
 }
 
-__device__ __forceinline__ uint4 philox(unsigned long long key, unsigned long long block, uint32_t stream, uint32_t h) {
-  uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = stream, c3 = h;
+// The words of N blocks.  The rounds of the blocks are interleaved: they share the key schedule and
+// fill each other's latency.
+template <int N>
+__device__ __forceinline__ void philox(unsigned long long key, const unsigned long long (&block)[N], uint32_t stream, uint32_t h,
+                                       uint32_t (&w)[N][4]) {
   uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
 #pragma unroll
+  for (int n = 0; n < N; ++n) {
+    w[n][0] = static_cast<uint32_t>(block[n]);
+    w[n][1] = static_cast<uint32_t>(block[n] >> 32);
+    w[n][2] = stream;
+    w[n][3] = h;
+  }
+#pragma unroll
   for (int r = 0; r < 10; ++r) {
-    const unsigned long long a = static_cast<unsigned long long>(0xD2511F53u) * c0;
-    const unsigned long long b = static_cast<unsigned long long>(0xCD9E8D57u) * c2;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(a);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const unsigned long long a = static_cast<unsigned long long>(0xD2511F53u) * w[n][0];
+      const unsigned long long b = static_cast<unsigned long long>(0xCD9E8D57u) * w[n][2];
+      w[n][0] = static_cast<uint32_t>(b >> 32) ^ w[n][1] ^ k0;
+      w[n][1] = static_cast<uint32_t>(b);
+      w[n][2] = static_cast<uint32_t>(a >> 32) ^ w[n][3] ^ k1;
+      w[n][3] = static_cast<uint32_t>(a);
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return make_uint4(c0, c1, c2, c3);
 }
 
-// The ties of a block, decided by the lower halves: one block in 8192, so it is kept out of line.
-static __device__ __noinline__ uint32_t keep8_ties(unsigned long long key, unsigned long long block, uint32_t stream, uint32_t last,
-                                            uint4 q) {
-  const uint4 s = philox(key, block, stream, 1);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w}, v[4] = {s.x, s.y, s.z, s.w};
-  uint32_t keep = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t hi = (w[j >> 1] >> (16 * (j & 1))) & 0xffffu, lo = (v[j >> 1] >> (16 * (j & 1))) & 0xffffu;
-    if (hi == (last >> 16) && lo > (last & 0xffffu)) keep |= 1u << j;
-  }
-  return keep;
-}
+// Which of a block's elements are dropped, as sign bits: bit 15 of d[j] for element 2j, bit 31 for
+// element 2j + 1 (the other bits mean nothing).
+//
+// The upper 15 bits of two numbers are compared with the limit's by one subtraction, whose borrow
+// bits are the answer unless a number ties; the most negative half, 0x8000, is the tie, so a running
+// minimum finds whether there is one.  Then (one block in 4096) the whole numbers are compared.
+struct Dropped { uint32_t d[4]; };
 
-// Bit j of the result: element 8 * block + j is kept.
-__device__ __forceinline__ uint32_t keep8(unsigned long long key, unsigned long long block, uint32_t stream, uint32_t last) {
-  const uint4 q = philox(key, block, stream, 0);
+static __device__ __noinline__ uint4 dropped_by_whole_numbers(unsigned long long key, unsigned long long block, uint32_t stream,
+                                                              uint32_t last, uint4 q) {
+  uint32_t low[1][4];
+  const unsigned long long one[1] = {block};
+  philox<1>(key, one, stream, 1, low);
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  const uint32_t top = last | 0xffffu;          // upper half above last's upper half <=> word > top
-  const uint32_t both = (last >> 16) * 0x10001u;
-  uint32_t keep = 0, tie = 0;
+  uint32_t d[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    keep |= ((w[j] << 16) > top ? 1u : 0u) << (2 * j);
-    keep |= (w[j] > top ? 2u : 0u) << (2 * j);
-    const uint32_t x = w[j] ^ both;             // a half that ties is zero here
-    tie |= (x - 0x10001u) & ~x & 0x80008000u;
+    const uint32_t even = w[j] << 16 | (low[0][j] & 0xffffu), odd = (w[j] & 0xffff0000u) | low[0][j] >> 16;
+    d[j] = (even <= last ? 0x8000u : 0u) | (odd <= last ? 0x80000000u : 0u);
   }
-  // `tie` is non-zero exactly when one of the eight halves ties
-  if (tie && (last & 0xffffu) != 0xffffu) keep |= keep8_ties(key, block, stream, last, q);
-  return keep;
+  return make_uint4(d[0], d[1], d[2], d[3]);
 }
 
-__device__ __forceinline__ bool kept(const Drop& d, unsigned long long key, unsigned long long i) {
-  return (keep8(key, i >> 3, d.stream, d.last) >> (i & 7)) & 1u;
+template <int N>
+__device__ __forceinline__ void dropped(const Drop& p, unsigned long long key, const unsigned long long (&block)[N], Dropped (&out)[N]) {
+  uint32_t w[N][4];
+  philox<N>(key, block, p.stream, 0, w);
+  const uint32_t limit = (p.last >> 17) * 0x10001u | 0x80008000u;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    uint32_t least = 0x7fff7fffu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      out[n].d[j] = limit - ((w[n][j] >> 1) & 0x7fff7fffu);
+      least = __vmins2(least, out[n].d[j]);
+    }
+    const uint32_t tie = least ^ 0x80008000u;      // a half that is zero
+    if (((tie - 0x10001u) & ~tie & 0x80008000u) && (p.last & 0x1ffffu) != 0x1ffffu) {
+      const uint4 d = dropped_by_whole_numbers(key, block[n], p.stream, p.last, make_uint4(w[n][0], w[n][1], w[n][2], w[n][3]));
+      out[n].d[0] = d.x; out[n].d[1] = d.y; out[n].d[2] = d.z; out[n].d[3] = d.w;
+    }
+  }
+}
+
+// All ones where element 0 / 1 of a pair is dropped, else zero.
+template <uint32_t SELECT>     // bytes 1 and 3 of d, their sign bits spread over bytes
+__device__ __forceinline__ uint32_t spread_signs(uint32_t d) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(d), "n"(SELECT));
+  return r;
+}
+__device__ __forceinline__ uint32_t sign_low(uint32_t d) { return spread_signs<0x9999>(d); }
+__device__ __forceinline__ uint32_t sign_high(uint32_t d) { return spread_signs<0xbbbb>(d); }
+__device__ __forceinline__ uint32_t sign_halves(uint32_t d) { return spread_signs<0xbb99>(d); }
+__device__ __forceinline__ float zero_if(float v, uint32_t mask) { return __uint_as_float(__float_as_uint(v) & ~mask); }
+
+// The sign bits of a block in one word, and back: unfold(x, j) stands for d[j].
+__device__ __forceinline__ uint32_t fold(const Dropped& f) {
+  return (f.d[0] & 0x80008000u) | (f.d[1] & 0x80008000u) >> 1 | (f.d[2] & 0x80008000u) >> 2 | (f.d[3] & 0x80008000u) >> 3;
+}
+__device__ __forceinline__ uint32_t unfold(uint32_t x, int j) { return x << j; }
+
+// One element at a time.
+__device__ __forceinline__ bool kept(const Drop& p, unsigned long long key, unsigned long long i) {
+  const unsigned long long one[1] = {i >> 3};
+  Dropped f[1];
+  dropped<1>(p, key, one, f);
+  return !(fold(f[0]) << ((i & 7) >> 1) & (i & 1 ? 0x80000000u : 0x8000u));
 }
 
 }  // namespace mb

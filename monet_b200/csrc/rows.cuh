@@ -22,7 +22,8 @@
 
 namespace mb {
 
-constexpr int kMaxThreads = 768;  // a CTA
+// Threads of a CTA: what the registers of an SM hold at 80 a thread, or 128 where a thread has 32 values.
+constexpr int kMaxThreads = 768, kMaxThreadsWide = 512;
 constexpr int kMaxTeam = 512;     // threads of a CTA that share a row
 constexpr int kUnit = 512;
 template <typename T> constexpr int kE = 16 / static_cast<int>(sizeof(T));    // elements of a granule
@@ -129,6 +130,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// 1 / v, off by one unit in the last place at most.
+__device__ __forceinline__ float reciprocal(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // ---- granules as pairs ---------------------------------------------------------------------
@@ -226,18 +233,28 @@ __device__ __forceinline__ void load_params(const void* p, bool is_f32, bool vec
   }
 }
 
-// Which elements of a granule (number `g` of the tensor) dropout keeps.
-template <typename T>
-__device__ __forceinline__ uint32_t keep_granule(const Drop& d, unsigned long long key, size_t g) {
-  if constexpr (kE<T> == 8) return keep8(key, g, d.stream, d.last);
-  else return (keep8(key, g >> 1, d.stream, d.last) >> (4 * (g & 1))) & 15u;
-}
-template <int N>
-__device__ __forceinline__ void apply_keep(float2 (&v)[N], uint32_t keep, float scale) {
+// What dropout does to N granules of the tensor (numbers g): sign bits as in Dropped, one word for
+// each pair of elements.
+template <typename T> struct Signs { uint32_t d[kPairs<T>]; };
+template <typename T, int N>
+__device__ __forceinline__ void granule_signs(const Drop& p, unsigned long long key, const size_t (&g)[N], Signs<T> (&out)[N]) {
+  unsigned long long block[N];
+  Dropped f[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i].x = (keep >> (2 * i)) & 1u ? __fmul_rn(v[i].x, scale) : 0.f;
-    v[i].y = (keep >> (2 * i)) & 2u ? __fmul_rn(v[i].y, scale) : 0.f;
+  for (int n = 0; n < N; ++n) block[n] = kE<T> == 8 ? g[n] : g[n] >> 1;
+  dropped<N>(p, key, block, f);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < kPairs<T>; ++i) out[n].d[i] = kE<T> == 8 || !(g[n] & 1) ? f[n].d[i] : f[n].d[i + 4 - kPairs<T>];
+}
+template <typename T, int P>
+__device__ __forceinline__ void apply_signs(float2 (&v)[P], const Signs<T>& s, float scale) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    v[i] = mul2(v[i], both(scale));
+    v[i].x = zero_if(v[i].x, sign_low(s.d[i]));
+    v[i].y = zero_if(v[i].y, sign_high(s.d[i]));
   }
 }
 template <int N>
