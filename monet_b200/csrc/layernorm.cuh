@@ -100,12 +100,17 @@ inline void plan_groups(size_t rows, int most, RowPlan* q) {
 
 // The ring beside `params` bytes: as many rows ahead as fit, up to eight; false if not even `least`
 // times the r rows between two barriers do.
-inline bool plan_ring(int r, int ops, int least, size_t params, RowPlan* q) {
+inline bool plan_ring(size_t rows, int r, int ops, int least, size_t params, RowPlan* q) {
   const size_t stage = static_cast<size_t>(ceil_div(q->groups * q->team, 32)) * q->per_thread * ops * kUnit;
   if (params >= kSmemLimit) return false;
   const size_t deep = (kSmemLimit - params) / (r * stage);
   if (deep < static_cast<size_t>(least)) return false;
-  q->stages = r * static_cast<int>(deep > static_cast<size_t>(8 / r) ? 8 / r : deep);
+  const size_t each = (rows + static_cast<size_t>(num_sms()) * q->groups - 1) / (static_cast<size_t>(num_sms()) * q->groups);
+  const size_t of_use = (each + r - 1) / r;                  // no more than a team has rows, if every SM has a CTA
+  int n = 8 / r;
+  if (deep < static_cast<size_t>(n)) n = static_cast<int>(deep);
+  if (of_use < static_cast<size_t>(n) && q->period == 1) n = static_cast<int>(of_use);
+  q->stages = r * n;
   q->smem = stage * q->stages + params;
   return true;
 }
@@ -138,7 +143,7 @@ inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from
     for (teams = q->team <= 32 || teams > fit ? fit : teams; teams >= 1; --teams) {
       plan_groups(rows, teams, q);
       const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
-      if (fold <= kSmemLimit && plan_ring(r, ops, 2, params, q)) {
+      if (fold <= kSmemLimit && plan_ring(rows, r, ops, 2, params, q)) {
         if (fold > q->smem) q->smem = fold;                  // the teams' column sums are folded there
         return true;
       }
@@ -162,7 +167,7 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
   for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
     plan_groups(rows, teams, q);
-    if (plan_ring(r, ops, teams == 1 ? 1 : 2, params, q)) return true;
+    if (plan_ring(rows, r, ops, teams == 1 ? 1 : 2, params, q)) return true;
   }
   return false;
 }

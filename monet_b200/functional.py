@@ -986,37 +986,35 @@ def depthwise_bwd(dy, x, w, stride, padding, dilation, groups, need=(True, True,
 
 # ------------------------------------------------------------- dropout and layer norm
 # These take float32, bfloat16 and float16 activations; arithmetic is fp32, results are rounded
-# once.  They run on the device of their first tensor, on that device's current stream.
+# once.  They run on the device of their first tensor, on that device's current stream.  A call on
+# a few rows is bound by this file rather than by its kernel: descriptors are built once per shape.
 
 from ._lib import DropoutDesc, LnDesc  # noqa: E402
 
 _DTYPE_CODE = {torch.float32: _lib.MB_F32, torch.bfloat16: _lib.MB_BF16, torch.float16: _lib.MB_F16}
+_F32 = torch.float32
 
 
-def _on_its_device(fn):
-    """Runs `fn` with the device of its first tensor as the current one."""
-    @functools.wraps(fn)
-    def call(t, *args, **kwargs):
-        if t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
-                return fn(t, *args, **kwargs)
-        return fn(t, *args, **kwargs)
-    return call
+def _current_device() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
 
 
-def _act_dtype(first: torch.Tensor, **others) -> int:
-    """The dtype code of `first`; every other (non-None) activation must match it in type and device."""
-    if not first.is_cuda:
+def _act_dtype(t: torch.Tensor) -> int:
+    """The dtype code of a CUDA activation."""
+    if not t.is_cuda:
         raise RuntimeError("monet_b200 operators run on CUDA tensors only (no CPU fallback)")
-    code = _DTYPE_CODE.get(first.dtype)
+    code = _DTYPE_CODE.get(t.dtype)
     if code is None:
-        raise RuntimeError(f"monet_b200: unsupported dtype {first.dtype} (float32, bfloat16, float16)")
-    for name, t in others.items():
-        if t is None:
-            continue
-        if t.dtype != first.dtype or t.device != first.device:
-            raise RuntimeError(f"monet_b200: {name} must be {first.dtype} on {first.device}, got {t.dtype} on {t.device}")
+        raise RuntimeError(f"monet_b200: unsupported dtype {t.dtype} (float32, bfloat16, float16)")
     return code
+
+
+def _alike(first: torch.Tensor, t: torch.Tensor, name: str) -> None:
+    if t.dtype != first.dtype or t.get_device() != first.get_device():
+        raise RuntimeError(f"monet_b200: {name} must be {first.dtype} on {first.device}, got {t.dtype} on {t.device}")
+    if t.shape != first.shape:
+        raise RuntimeError(f"monet_b200: {name} must have the shape {tuple(first.shape)}, got {tuple(t.shape)} "
+                           "(broadcasting is not supported)")
 
 
 def dropout_seed(device) -> torch.Tensor:
@@ -1027,19 +1025,20 @@ def dropout_seed(device) -> torch.Tensor:
 
 def _drop_desc(x: torch.Tensor, p: float, seed, offset: int):
     """(descriptor or None when nothing is dropped); checks the seed."""
-    p = float(p)
     if not 0.0 <= p <= 1.0:
         raise RuntimeError(f"monet_b200: dropout probability must lie in [0, 1], got {p}")
     if p * 2.0 ** 32 < 0.5:
         return None
     if not (torch.is_tensor(seed) and seed.dtype == torch.int64 and seed.numel() == 1 and seed.device == x.device):
         raise RuntimeError(f"monet_b200: the dropout seed must be an int64 tensor of one element on {x.device}")
-    if not 0 <= int(offset) < 2 ** 32:
+    if not 0 <= offset < 2 ** 32:
         raise RuntimeError(f"monet_b200: dropout offset must lie in [0, 2^32), got {offset}")
-    return DropoutDesc(p, seed.data_ptr(), int(offset))
+    return DropoutDesc(p, seed.data_ptr(), offset)
 
 
-@_on_its_device
+_NO_DROPOUT = DropoutDesc(0.0, None, 0)
+
+
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool = False) -> torch.Tensor:
     """x / (1 - p) where kept, 0 where dropped.  Which elements are dropped depends on `seed` (an
     int64 tensor of one element on x's device, ``dropout_seed``), `offset` (tells dropouts that
@@ -1047,7 +1046,10 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool = Fa
     ``dropout_bwd`` and a repeated forward draw the same one.  The generator is specified at
     ``mb_dropout`` in the header."""
     code = _act_dtype(x)
-    desc = _drop_desc(x, p, seed, offset) or DropoutDesc(0.0, None, 0)
+    if x.get_device() != _current_device():
+        with torch.cuda.device(x.device):
+            return dropout(x, p, seed, offset, inplace)
+    desc = _drop_desc(x, p, seed, offset) or _NO_DROPOUT
     xd = dense(x)
     y = xd if (inplace and xd is x) else torch.empty_like(xd)
     check(lib().mb_dropout(xd.data_ptr(), y.data_ptr(), xd.numel(), code, C.byref(desc), _stream()), "dropout")
@@ -1060,15 +1062,26 @@ def dropout_bwd(dy: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool
     return dropout(dy, p, seed, offset, inplace)
 
 
-def _norm_geometry(x: torch.Tensor, normalized_shape):
-    """(rows, cols) of x seen as rows of the trailing dimensions `normalized_shape`."""
-    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(s) for s in normalized_shape)
-    if not shape or x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
-        raise RuntimeError(f"monet_b200: normalized_shape {shape} is not the end of the input's shape {tuple(x.shape)}")
-    cols = math.prod(shape)
+@functools.lru_cache(maxsize=4096)
+def _norm_geometry(shape, normalized_shape):
+    """(rows, cols, parameter shape) of a tensor seen as rows of its trailing dimensions."""
+    tail = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(s) for s in normalized_shape)
+    if not tail or len(shape) < len(tail) or tuple(shape[len(shape) - len(tail):]) != tail:
+        raise RuntimeError(f"monet_b200: normalized_shape {tail} is not the end of the input's shape {tuple(shape)}")
+    cols = math.prod(tail)
     if cols == 0:
         raise RuntimeError("monet_b200: layer norm over zero values")
-    return x.numel() // cols, cols
+    return math.prod(shape) // cols, cols, tail
+
+
+@functools.lru_cache(maxsize=4096)
+def _ln_desc(rows, cols, ld_a, ld_b, ld_c, code, param_code, eps):
+    return LnDesc(rows, cols, ld_a, ld_b, ld_c, code, param_code, eps)
+
+
+@functools.lru_cache(maxsize=4096)
+def _ln_workspace(device, rows, cols, code, param_code) -> int:
+    return lib().mb_layer_norm_workspace_bytes(C.byref(_ln_desc(rows, cols, cols, cols, cols, code, param_code, 0.0)))
 
 
 def _as_rows(t: torch.Tensor, rows: int, cols: int):
@@ -1084,21 +1097,26 @@ def _as_rows(t: torch.Tensor, rows: int, cols: int):
     return v, v.stride(0) if rows > 1 else cols
 
 
-def _norm_params(x: torch.Tensor, cols: int, code: int, weight, bias):
-    """(weight, bias, dtype code) made dense; they are fp32 or of x's type, and alike."""
-    kind = None
-    out = []
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.device != x.device or t.numel() != cols:
-                raise RuntimeError(f"monet_b200: {name} must have {cols} values on {x.device}")
-            if t.dtype not in (torch.float32, x.dtype) or (kind is not None and t.dtype != kind):
-                raise RuntimeError(f"monet_b200: weight and bias must both be float32 or both {x.dtype}, got {name} {t.dtype}")
-            kind = t.dtype
-            t = t.detach()
-            t = t if t.is_contiguous() else t.contiguous()
-        out.append(t)
-    return out[0], out[1], _lib.MB_F32 if kind in (None, torch.float32) else code
+def _norm_param(x: torch.Tensor, cols: int, t, name: str):
+    if t.get_device() != x.get_device() or t.numel() != cols:
+        raise RuntimeError(f"monet_b200: {name} must have {cols} values on {x.device}")
+    if t.dtype != _F32 and t.dtype != x.dtype:
+        raise RuntimeError(f"monet_b200: {name} must be float32 or {x.dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else t.detach().contiguous()
+
+
+def _norm_params(x: torch.Tensor, cols: int, weight, bias):
+    """(weight, bias, their dtype) made dense; they are fp32 or of x's type, and alike."""
+    kind = _F32
+    if weight is not None:
+        weight = _norm_param(x, cols, weight, "weight")
+        kind = weight.dtype
+    if bias is not None:
+        bias = _norm_param(x, cols, bias, "bias")
+        if weight is not None and bias.dtype != kind:
+            raise RuntimeError(f"monet_b200: weight and bias must have one type, got {kind} and {bias.dtype}")
+        kind = bias.dtype
+    return weight, bias, kind
 
 
 def _ptr(t):
@@ -1106,95 +1124,111 @@ def _ptr(t):
 
 
 def _row_stat(t: torch.Tensor, x: torch.Tensor, rows: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.float32 or t.device != x.device or t.numel() != rows:
+    if t.dtype != _F32 or t.get_device() != x.get_device() or t.numel() != rows:
         raise RuntimeError(f"monet_b200: {name} must hold {rows} float32 values on {x.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, drop, want_sum, inplace):
-    code = _act_dtype(x, residual=residual)
-    rows, cols = _norm_geometry(x, normalized_shape)
-    if residual is not None and residual.shape != x.shape:
-        raise RuntimeError("monet_b200: residual and input shapes differ (broadcasting is not supported)")
-    w, b, pcode = _norm_params(x, cols, code, weight, bias)
-    xr, lda = _as_rows(x, rows, cols)
-    rr, ldb = _as_rows(residual, rows, cols) if residual is not None else (None, 0)
-    y = x if inplace and x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_sum else None
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
-    d = LnDesc(rows, cols, lda, ldb, 0, code, pcode, float(eps))
-    check(lib().mb_layer_norm_fwd(xr.data_ptr(), _ptr(rr), _ptr(w), _ptr(b), y.data_ptr(), _ptr(z),
-                                  mean.data_ptr(), rstd.data_ptr(), C.byref(d),
-                                  C.byref(drop) if drop is not None else None, _stream()), "layer_norm_fwd")
+def _hashable(normalized_shape):
+    return normalized_shape if isinstance(normalized_shape, (int, tuple)) else tuple(normalized_shape)
+
+
+def _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, p, seed, offset, want_sum, inplace):
+    code = _act_dtype(x)
+    if x.get_device() != _current_device():
+        with torch.cuda.device(x.device):
+            return _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, p, seed, offset, want_sum, inplace)
+    drop = _drop_desc(x, p, seed, offset) if residual is not None else None
+    rows, cols, _ = _norm_geometry(x.shape, _hashable(normalized_shape))
+    w, b, kind = _norm_params(x, cols, weight, bias)
+    xr, ld_a = _as_rows(x, rows, cols)
+    rr, ld_b = None, 0
+    if residual is not None:
+        _alike(x, residual, "residual")
+        rr, ld_b = _as_rows(residual, rows, cols)
+    if xr is not x:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        y = x if inplace else torch.empty_like(x)
+    z = torch.empty_like(y) if want_sum else None
+    mean = torch.empty(rows, dtype=_F32, device=x.device)
+    rstd = torch.empty(rows, dtype=_F32, device=x.device)
+    d = _ln_desc(rows, cols, ld_a, ld_b, 0, code, _DTYPE_CODE[kind], eps)
+    check(lib().mb_layer_norm_fwd(xr.data_ptr(), _ptr(rr), _ptr(w), _ptr(b), y.data_ptr(), _ptr(z), mean.data_ptr(),
+                                  rstd.data_ptr(), C.byref(d), C.byref(drop) if drop is not None else None, _stream()),
+          "layer_norm_fwd")
     return y, z, mean, rstd
 
 
-def _layer_norm_bwd(dy, kept, from_output, dz, normalized_shape, weight, bias, mean, rstd, drop,
+def _layer_norm_bwd(dy, kept, from_output, dz, normalized_shape, weight, bias, mean, rstd, p, seed, offset,
                     need_weight, need_bias):
-    code = _act_dtype(dy, kept=kept, dz=dz)
-    rows, cols = _norm_geometry(kept, normalized_shape)
-    if dy.shape != kept.shape or (dz is not None and dz.shape != kept.shape):
-        raise RuntimeError("monet_b200: gradient and activation shapes differ")
-    w, b, pcode = _norm_params(kept, cols, code, weight, bias)
+    code = _act_dtype(dy)
+    if dy.get_device() != _current_device():
+        with torch.cuda.device(dy.device):
+            return _layer_norm_bwd(dy, kept, from_output, dz, normalized_shape, weight, bias, mean, rstd, p, seed, offset,
+                                   need_weight, need_bias)
+    drop = _drop_desc(dy, p, seed, offset)
+    rows, cols, tail = _norm_geometry(dy.shape, _hashable(normalized_shape))
+    _alike(dy, kept, "the kept activation")
+    w, b, kind = _norm_params(dy, cols, weight, bias)
     rstd = _row_stat(rstd, dy, rows, "rstd")
     mean = _row_stat(mean, dy, rows, "mean") if mean is not None else None
-    gr, lda = _as_rows(dy, rows, cols)
-    kr, ldb = _as_rows(kept, rows, cols)
-    zr, ldc = _as_rows(dz, rows, cols) if dz is not None else (None, 0)
-    device = dy.device
-    dv = torch.empty(dy.shape, dtype=dy.dtype, device=device)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=device) if drop is not None else None
-    pdtype = torch.float32 if pcode == _lib.MB_F32 else dy.dtype
-    pshape = tuple(kept.shape[kept.dim() - (1 if isinstance(normalized_shape, int) else len(normalized_shape)):])
-    dw = torch.empty(pshape, dtype=pdtype, device=device) if need_weight else None
-    db = torch.empty(pshape, dtype=pdtype, device=device) if need_bias else None
-    d = LnDesc(rows, cols, lda, ldb, ldc, code, pcode, 0.0)
-    nbytes = lib().mb_layer_norm_workspace_bytes(C.byref(d)) if need_weight or need_bias else 0
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
-    check(lib().mb_layer_norm_bwd(gr.data_ptr(), kr.data_ptr(), int(from_output), _ptr(zr), _ptr(w), _ptr(b),
-                                  _ptr(mean), rstd.data_ptr(), dv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                                  C.byref(d), C.byref(drop) if drop is not None else None,
-                                  ws.data_ptr(), ws.numel(), _stream()), "layer_norm_bwd")
+    # the fast kernels take dense rows, and a copy costs less than the element-wise ones
+    gr, kr, zr = dy.contiguous(), kept.contiguous(), None
+    if dz is not None:
+        _alike(dy, dz, "dz")
+        zr = dz.contiguous()
+    dv = torch.empty_like(gr)
+    dx = torch.empty_like(gr) if drop is not None else None
+    dw = torch.empty(tail, dtype=kind, device=dy.device) if need_weight else None
+    db = torch.empty(tail, dtype=kind, device=dy.device) if need_bias else None
+    pcode = _DTYPE_CODE[kind]
+    ws, nbytes = None, 0
+    if need_weight or need_bias:
+        nbytes = _ln_workspace(dy.get_device(), rows, cols, code, pcode)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+    d = _ln_desc(rows, cols, cols, cols, cols, code, pcode, 0.0)
+    check(lib().mb_layer_norm_bwd(gr.data_ptr(), kr.data_ptr(), from_output, _ptr(zr), _ptr(w), _ptr(b), _ptr(mean),
+                                  rstd.data_ptr(), dv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), C.byref(d),
+                                  C.byref(drop) if drop is not None else None, _ptr(ws), nbytes, _stream()), "layer_norm_bwd")
     return dv, dx, dw, db
 
 
-@_on_its_device
 def layer_norm(x: torch.Tensor, normalized_shape, weight=None, bias=None, eps: float = 1e-5, inplace: bool = False):
     """(y, mean, rstd): layer norm over the trailing dimensions `normalized_shape`; mean and rstd
     (= 1/sqrt(biased variance + eps)) are fp32, one value a row.  `weight` and `bias` are fp32 or of
-    x's type.  `inplace` overwrites a contiguous x."""
-    y, _, mean, rstd = _layer_norm_fwd(x, None, normalized_shape, weight, bias, eps, None, False, inplace)
+    x's type.  `inplace` overwrites a contiguous x.  A row's result does not depend on how many
+    other rows there are."""
+    y, _, mean, rstd = _layer_norm_fwd(x, None, normalized_shape, weight, bias, eps, 0.0, None, 0, False, inplace)
     return y, mean, rstd
 
 
-@_on_its_device
 def layer_norm_bwd_from_input(dy, x, normalized_shape, weight, mean, rstd, need_weight: bool = True, need_bias: bool = True):
     """(dx, dweight, dbias) from the stored INPUT; the parameters' gradients have the weight's type
     (fp32 without one) and are None when not needed."""
-    dx, _, dw, db = _layer_norm_bwd(dy, x, False, None, normalized_shape, weight, None, mean, rstd, None,
+    dx, _, dw, db = _layer_norm_bwd(dy, x, 0, None, normalized_shape, weight, None, mean, rstd, 0.0, None, 0,
                                     need_weight, need_bias)
     return dx, dw, db
 
 
-@_on_its_device
 def layer_norm_bwd_from_output(dy, y, normalized_shape, weight, bias, rstd, need_weight: bool = True, need_bias: bool = True):
     """(dx, dweight, dbias) from the stored OUTPUT, xhat = (y - bias) / weight: the input need not
-    be kept and the forward can run in place.  A weight of zero is undefined (NaN), as for batch norm,
-    and y's rounding enters xhat divided by the weight."""
-    dx, _, dw, db = _layer_norm_bwd(dy, y, True, None, normalized_shape, weight, bias, None, rstd, None,
+    be kept and the forward can run in place.  A weight of zero is undefined, as for batch norm (NaN or
+    infinite gradients in its column), and y's rounding enters xhat divided by the weight."""
+    dx, _, dw, db = _layer_norm_bwd(dy, y, 1, None, normalized_shape, weight, bias, None, rstd, 0.0, None, 0,
                                     need_weight, need_bias)
     return dx, dw, db
 
 
-@_on_its_device
 def dropout_add_layer_norm(x, residual, normalized_shape, weight=None, bias=None, eps: float = 1e-5, p: float = 0.0,
                            seed=None, offset: int = 0, want_sum: bool = True, inplace: bool = False):
     """(y, z, mean, rstd) with z = residual + dropout(x) and y = layer_norm(z), in one pass.  The
     dropout is ``dropout``'s with the element's row-major index; z is None unless `want_sum` (a
-    pre-norm network carries it on; its statistics are those of the unrounded sum)."""
-    drop = _drop_desc(x, p, seed, offset)
-    return _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, drop, want_sum, inplace)
+    pre-norm network carries it on; the statistics are those of the unrounded sum).  `inplace`
+    writes y over a contiguous x."""
+    if residual is None:
+        raise RuntimeError("monet_b200.dropout_add_layer_norm needs a residual")
+    return _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, p, seed, offset, want_sum, inplace)
 
 
 def _pair_of_gradients(dv, dx, dw, db):
@@ -1202,20 +1236,16 @@ def _pair_of_gradients(dv, dx, dw, db):
     return (dv if dx is None else dx), dv, dw, db
 
 
-@_on_its_device
 def dropout_add_layer_norm_bwd_from_sum(dy, z, normalized_shape, weight, mean, rstd, p: float = 0.0, seed=None,
                                         offset: int = 0, dz=None, need_weight: bool = True, need_bias: bool = True):
     """(dx, dresidual, dweight, dbias) from the stored SUM z; `dz` is the gradient that z receives
     from elsewhere.  dx is dresidual itself when nothing is dropped."""
-    drop = _drop_desc(dy, p, seed, offset)
-    return _pair_of_gradients(*_layer_norm_bwd(dy, z, False, dz, normalized_shape, weight, None, mean, rstd, drop,
+    return _pair_of_gradients(*_layer_norm_bwd(dy, z, 0, dz, normalized_shape, weight, None, mean, rstd, p, seed, offset,
                                                need_weight, need_bias))
 
 
-@_on_its_device
 def dropout_add_layer_norm_bwd_from_output(dy, y, normalized_shape, weight, bias, rstd, p: float = 0.0, seed=None,
                                            offset: int = 0, dz=None, need_weight: bool = True, need_bias: bool = True):
     """The same from the stored OUTPUT y, xhat = (y - bias) / weight (``layer_norm_bwd_from_output``)."""
-    drop = _drop_desc(dy, p, seed, offset)
-    return _pair_of_gradients(*_layer_norm_bwd(dy, y, True, dz, normalized_shape, weight, bias, None, rstd, drop,
+    return _pair_of_gradients(*_layer_norm_bwd(dy, y, 1, dz, normalized_shape, weight, bias, None, rstd, p, seed, offset,
                                                need_weight, need_bias))
