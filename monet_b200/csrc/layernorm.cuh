@@ -119,8 +119,8 @@ inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from
   if (rows >> 30) return false;                              // row numbers are 32-bit, and some steps ahead
   const int elems = 16 / elem;
   const size_t most = row_granules(cols, elems, &q->period);
-  if (most > static_cast<size_t>(kMaxTeam) * 8 * (32 / elems)) return false;
-  for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
+  if (most > static_cast<size_t>(kMaxTeam) * kMaxCluster * (32 / elems)) return false;
+  for (q->cluster = 1; q->cluster <= kMaxCluster; q->cluster *= 2) {
     const int chunk = ceil_div(static_cast<long long>(most), q->cluster);
     // the fp32 weight (with from_y also minus the bias) lies beside the ring
     const size_t params_row = static_cast<size_t>(chunk) * elems * 4 * (from_y ? 2 : 1), row = static_cast<size_t>(chunk) * 16 * ops;
@@ -143,7 +143,7 @@ inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from
     for (teams = q->team <= 32 || teams > fit ? fit : teams; teams >= 1; --teams) {
       plan_groups(rows, teams, q);
       const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
-      if (fold <= kSmemLimit && plan_ring(rows, r, ops, 2, params, q)) {
+      if (fold <= kSmemLimit && plan_ring(rows, r, ops, q->cluster == kMaxCluster ? 1 : 2, params, q)) {
         if (fold > q->smem) q->smem = fold;                  // the teams' column sums are folded there
         return true;
       }
@@ -156,18 +156,21 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   if (rows >> 30) return false;
   const int elems = 16 / elem;
   const size_t most = row_granules(cols, elems, &q->period);
-  q->cluster = 1;
-  if (most > static_cast<size_t>(kMaxTeam) * (32 / elems)) return false;
-  const int chunk = static_cast<int>(most);
-  int values = one_warp_values(chunk, elems);
-  if (!values) values = 32;      // (16384 x 8192 bf16: 115 us against 154 with 16)
-  plan_team(chunk, elems, values, q);
-  if (q->team > kMaxTeam) return false;
-  const int r = fwd_rows_between_barriers(q->per_thread, elems);
-  const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
-  for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
-    plan_groups(rows, teams, q);
-    if (plan_ring(rows, r, ops, teams == 1 ? 1 : 2, params, q)) return true;
+  if (most > static_cast<size_t>(kMaxTeam) * kMaxCluster * (32 / elems)) return false;
+  for (q->cluster = 1; q->cluster <= kMaxCluster; q->cluster *= 2) {
+    const int chunk = ceil_div(static_cast<long long>(most), q->cluster);
+    int values = q->cluster > 1 ? 0 : one_warp_values(chunk, elems);
+    if (!values) values = 32;      // (16384 x 8192 bf16: 115 us against 154 with 16)
+    // a cluster's CTA has one team, so it takes as many threads as it can
+    if (q->cluster > 1 && chunk * elems <= 16 * kMaxThreads) values = 16;
+    plan_team(chunk, elems, values, q);
+    if (q->team > (values == 16 && q->cluster > 1 ? kMaxThreads : kMaxTeam)) continue;
+    const int r = fwd_rows_between_barriers(q->per_thread, elems);
+    const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
+    for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
+      plan_groups(rows, teams, q);
+      if (plan_ring(rows, r, ops, 2, params, q)) return true;
+    }
   }
   return false;
 }
@@ -213,6 +216,7 @@ int prepare(const char* who, Kernel kernel, std::atomic<int>* cache, int* regs) 
   if (r == 0) {
     cudaFuncAttributes a;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return fail(MB_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(cudaGetLastError()));
     r = a.numRegs + 1;
@@ -249,10 +253,10 @@ int launch_rows(const char* who, void (*kernel)(KArgs...), const RowPlan& q, cud
 }
 
 // A cluster's CTAs run together: a grid of more clusters than fit at once would end in a second,
-// nearly empty round.
+// nearly empty round.  False if not even one fits this device.
 template <typename Kernel>
-void fit_clusters(Kernel kernel, RowPlan* q) {
-  if (q->cluster == 1) return;
+bool fit_clusters(Kernel kernel, RowPlan* q) {
+  if (q->cluster == 1) return true;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(q->grid);
   cfg.blockDim = dim3(q->groups * q->team);
@@ -264,13 +268,13 @@ void fit_clusters(Kernel kernel, RowPlan* q) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return;
-  }
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) cudaGetLastError();
+  if (n < 1) return false;
   n -= n % q->period;
   if (n >= q->period && q->grid > n * q->cluster) q->grid = n * q->cluster;
+  return true;
 }
+constexpr int kDoesNotFit = -1;      // not a status: the caller takes another kernel
 
 int check_desc(const char* who, const mb_ln_desc* d) {
   if (!d) return fail(MB_ERR_INVALID_ARGUMENT, "%s: null descriptor", who);

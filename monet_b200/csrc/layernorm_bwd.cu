@@ -18,7 +18,7 @@ template <typename T, int K, int R, bool FROM_Y, bool DSUM, bool DROP, bool EDGE
 __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float red[2][kMaxThreads / 32][2 * R];      // double-buffered by row: one barrier a row
-  __shared__ float peer[2][8][2 * R];
+  __shared__ float peer[2][kMaxCluster][2 * R];
   if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
   constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 2 : 1;
   constexpr int kParam = kParamUnits<T> * kUnit;
@@ -44,12 +44,13 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   // byte offset of the thread's first granule in the first of the rows at hand (all tensors are dense)
   size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, j0) * sizeof(T);
   const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
-  auto fetch = [&](uint32_t stage, size_t off) {
+  const int ends = last_rows<T, EDGE>(rows, p.cols);
+  auto fetch = [&](uint32_t stage, int i, size_t off) {
 #pragma unroll
     for (int o = 0; o < kOps; ++o)
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (mask[k]) ring_copy<EDGE>(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, p.rows * p.cols * sizeof(T));
+        if (mask[k]) ring_copy(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, EDGE && i >= ends, p.rows * p.cols * sizeof(T));
   };
 
   float2 wr[P], nbr[P];                // kInRegs: the weight; with FROM_Y minus the bias
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   for (int s = 0; s < q.stages; s += R) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (at.first + (s + r) * step < rows) fetch(slots + (s + r) * stride, out + (s + r) * out_step);
+      if (at.first + (s + r) * step < rows) fetch(slots + (s + r) * stride, at.first + (s + r) * step, out + (s + r) * out_step);
     cp_async_commit();
   }
   if (kInRegs || at.group == 0) {
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     // the next rows into the slots just read for the last time
 #pragma unroll
     for (int r = 0; r < R; ++r)
-      if (row + (q.stages + r) * step < rows) fetch(stage + r * stride, out + (q.stages + r) * out_step);
+      if (row + (q.stages + r) * step < rows) fetch(stage + r * stride, row + (q.stages + r) * step, out + (q.stages + r) * out_step);
     cp_async_commit();
     stage += R * stride;
     if (stage >= slots + q.stages * stride) stage = slots;
@@ -436,7 +437,7 @@ int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
   auto kernel = ln_bwd_rows<T, K, bwd_rows_between_barriers(K), FROM_Y, DSUM, DROP, EDGE, CLUSTER>;
   int regs = 0;
   if (int rc = prepare("layer_norm_bwd", kernel, cache, &regs)) return rc;
-  fit_clusters(kernel, &q);
+  if (!fit_clusters(kernel, &q)) return kDoesNotFit;
   const bool sums = g.dw || g.db;
   if (int rc = launch_rows("layer_norm_bwd", kernel, q, st, p, q, sums ? g.ws : nullptr)) return rc;
   return sums ? finish<T>(g.ws, q.grid / q.cluster, p.cols, g.dw, g.db, p.w_f32, st) : MB_OK;
@@ -464,8 +465,10 @@ int bwd(const LnArgs& p, const mb_ln_desc* d, bool granules, const Grads& g, cud
   RowPlan q;
   // (a dx that equals dv because nothing is dropped is rare enough for the element-wise kernels)
   if (granules && (p.drop.on || !p.out2) && plan_bwd(d, p.c ? 3 : 2, FROM_Y, &q)) {
-    if (p.drop.on) return p.c ? pick_edge<T, FROM_Y, true, true>(p, q, g, st) : pick_edge<T, FROM_Y, false, true>(p, q, g, st);
-    return p.c ? pick_edge<T, FROM_Y, true, false>(p, q, g, st) : pick_edge<T, FROM_Y, false, false>(p, q, g, st);
+    int rc;
+    if (p.drop.on) rc = p.c ? pick_edge<T, FROM_Y, true, true>(p, q, g, st) : pick_edge<T, FROM_Y, false, true>(p, q, g, st);
+    else rc = p.c ? pick_edge<T, FROM_Y, true, false>(p, q, g, st) : pick_edge<T, FROM_Y, false, false>(p, q, g, st);
+    if (rc != kDoesNotFit) return rc;
   }
   if (g.dw || g.db) {      // before the outputs, which may lie over the inputs
     const int parts = column_parts(d);

@@ -5,10 +5,10 @@ namespace mb {
 namespace {
 
 // ---- rows in registers -----------------------------------------------------------------------
-// Statistics: every warp centres on its own mean, and the warps' (count, sum, squared deviations)
-// are combined, so no difference of large sums is ever formed.  R rows share the shuffles and the
-// barrier of a reduction, which are what a row of a few hundred values waits for.
-
+// Statistics: every thread centres on its own mean, and (sum, squared deviations) are merged pairwise
+// over the lanes, then over the warps and the CTAs of a cluster: no difference of large sums is ever
+// formed, and one pass over the lanes does.  (Where a warp's lanes hold different numbers of values it
+// centres on the warp's mean instead.)
 template <int P>
 __device__ __forceinline__ void normalise(float2 (&y)[P], float mean, float rstd, const float2 (&w)[P], const float2 (&b)[P]) {
 #pragma unroll
@@ -25,11 +25,13 @@ __device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, u
   return sum;
 }
 
-template <typename T, int K, int R, bool RES, bool EDGE>
+template <typename T, int K, int R, bool RES, bool EDGE, bool CLUSTER>
 __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
   __shared__ float counts[kMaxThreads / 32];
+  __shared__ float peer[2][kMaxCluster][3];
+  if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
   constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1, kSlots = K * kOps;
   constexpr int kParam = kParamUnits<T> * kUnit;
   constexpr uint32_t kAll = (1u << E) - 1;
@@ -50,23 +52,26 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     mask[k] = column_mask<T, EDGE>(at, q, at.t + k * q.team, p.cols);
     count += static_cast<float>(__popc(mask[k]));
   }
+  const int j0 = at.rank * q.chunk + at.t;           // the thread's granules: j0 + k * team
+  const bool even = __all_sync(0xffffffffu, count == static_cast<float>(K * E));      // the warp's lanes have equal counts
   if (!kInRegs) {
     count = warp_sum(count);
     if (lane == 0) counts[threadIdx.x >> 5] = count;
   }
 
-  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, at.t) * sizeof(T);
+  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, j0) * sizeof(T);
   const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
   // inputs may have gaps between their rows
-  size_t in_a = row_offset<T, EDGE>(at.first, p.ld_a, p.cols, at.t) * sizeof(T), in_b = RES ? row_offset<T, EDGE>(at.first, p.ld_b, p.cols, at.t) * sizeof(T) : 0;
+  size_t in_a = row_offset<T, EDGE>(at.first, p.ld_a, p.cols, j0) * sizeof(T), in_b = RES ? row_offset<T, EDGE>(at.first, p.ld_b, p.cols, j0) * sizeof(T) : 0;
   int next = at.first;
+  const int ends = last_rows<T, EDGE>(rows, p.cols);
   auto fetch = [&](uint32_t stage) {
     if (next < rows) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!mask[k]) continue;
-        ring_copy<EDGE>(stage + (k * kOps) * kUnit, p.a, in_a + k * kstep, p.rows * p.cols * sizeof(T));
-        if (RES) ring_copy<EDGE>(stage + (k * kOps + 1) * kUnit, p.b, in_b + k * kstep, p.rows * p.cols * sizeof(T));
+        ring_copy(stage + (k * kOps) * kUnit, p.a, in_a + k * kstep, EDGE && next >= ends, p.rows * p.cols * sizeof(T));
+        if (RES) ring_copy(stage + (k * kOps + 1) * kUnit, p.b, in_b + k * kstep, EDGE && next >= ends, p.rows * p.cols * sizeof(T));
       }
       in_a += static_cast<size_t>(step) * p.ld_a * sizeof(T);
       if (RES) in_b += static_cast<size_t>(step) * p.ld_b * sizeof(T);
@@ -89,7 +94,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   if (kInRegs || at.group == 0) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const long long col = static_cast<long long>(at.t + k * q.team) * E - at.m;
+      const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
       load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, wr);
       load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, br);
       if (!kInRegs) {
@@ -99,10 +104,12 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     }
   }
   if (!kInRegs) __syncthreads();       // the parameters that group 0 put down, and the counts
-  // combining the warps' statistics, this lane looks after row lane % R of warp lane / R
-  const int part = lane / R;
-  const float part_count = q.team > 32 && part < warps ? counts[at.group * warps + part] : 0.f;
-  const float part_inv = part_count > 0.f ? 1.f / part_count : 0.f;
+  // Combining the warps' statistics, a lane looks after the warp of its number.  Warps with equal counts,
+  // a power of two of them, merge like lanes.
+  const bool alike = !EDGE && q.chunk == K * q.team && (warps & (warps - 1)) == 0;
+  const float part_count = q.team > 32 && lane < warps ? counts[at.group * warps + lane] : 0.f;
+  const float part_inv = part_count > 0.f ? 1.f / part_count : 0.f, part_total = q.team > 32 ? warp_sum(part_count) : 0.f;
+  const float part_each = part_total > 0.f ? 1.f / part_total : 0.f;
 
   uint32_t stage = slots;
   int row = at.first, buf = 0;
@@ -144,49 +151,72 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     if (stage >= slots + q.stages * stride) stage = slots;
 
     float mean[R], m2[R];
-    auto spread = [&](const float (&centre)[R], float (&d)[R]) {
+    auto spread = [&](const float (&centre)[R], bool whole) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float2 sum = both(0.f);
 #pragma unroll
-        for (int k = 0; k < K; ++k) sum = deviations(v[r][k], centre[r], mask[k], mask[k] == kAll, sum);
-        d[r] = sum.x + sum.y;
+        for (int k = 0; k < K; ++k) sum = deviations(v[r][k], centre[r], mask[k], whole || mask[k] == kAll, sum);
+        m2[r] = sum.x + sum.y;
       }
     };
-    if (q.team <= 32) {
-      lanes_sums(s, q.team);
+    if (even && !kInRegs) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) mean[r] = s[r] * inv_n;
-      spread(mean, m2);
-      lanes_sums(m2, q.team);
+      for (int r = 0; r < R; ++r) mean[r] = s[r] * (1.f / (K * E));
+      spread(mean, true);
+      merge_lanes(s, m2, q.team < 32 ? q.team : 32, static_cast<float>(K * E));
     } else {
-      const float x = warp_sums(s);
+      const float each = kInRegs ? inv_n : count > 0.f ? 1.f / count : 0.f;
+      lanes_sums(s, kInRegs ? q.team : 32);
 #pragma unroll
-      for (int r = 0; r < R; ++r) mean[r] = count > 0.f ? __shfl_sync(0xffffffffu, x, r * (32 / R)) / count : 0.f;
-      spread(mean, m2);
-      const float y = warp_sums(m2);
-      if ((lane & (32 / R - 1)) == 0) red[buf][threadIdx.x >> 5][lane / (32 / R)] = make_float2(x, y);
+      for (int r = 0; r < R; ++r) mean[r] = s[r] * each;
+      spread(mean, false);
+      lanes_sums(m2, kInRegs ? q.team : 32);
+    }
+    if (q.team > 32) {
+      if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r) red[buf][threadIdx.x >> 5][r] = make_float2(s[r], m2[r]);
       team_barrier(at.group, q.team);
-      const float2 f = part < warps ? red[buf][at.group * warps + part][lane % R] : make_float2(0.f, 0.f);
-      float sum = f.x;
-#pragma unroll
-      for (int o = R; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      sum *= inv_n;
-      const float d = f.x * part_inv - sum;
-      float sq = part_count > 0.f ? fmaf(part_count * d, d, f.y) : 0.f;
-#pragma unroll
-      for (int o = R; o < 32; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        mean[r] = R == 1 ? sum : __shfl_sync(0xffffffffu, sum, r);
-        m2[r] = R == 1 ? sq : __shfl_sync(0xffffffffu, sq, r);
+        const float2(*f)[R] = red[buf] + at.group * warps;
+        float total, sq, n = part_total;
+        if (alike) {
+          float ts[1] = {f[lane & (warps - 1)][r].x}, tq[1] = {f[lane & (warps - 1)][r].y};
+          merge_lanes(ts, tq, warps, static_cast<float>(32 * K * E));
+          total = ts[0];
+          sq = tq[0];
+        } else {
+          const float2 mine = lane < warps ? f[lane][r] : make_float2(0.f, 0.f);
+          total = warp_sum(mine.x);
+          const float d = mine.x * part_inv - total * part_each;
+          sq = warp_sum(part_inv > 0.f ? fmaf(part_count * d, d, mine.y) : 0.f);
+        }
+        if (CLUSTER) {
+          if (threadIdx.x < q.cluster) {
+            put_remote(&peer[buf][at.rank][0], threadIdx.x, total);
+            put_remote(&peer[buf][at.rank][1], threadIdx.x, sq);
+            put_remote(&peer[buf][at.rank][2], threadIdx.x, n);
+          }
+          cluster_barrier();
+          const bool have = lane < q.cluster;
+          const float ps = have ? peer[buf][lane][0] : 0.f, pq = have ? peer[buf][lane][1] : 0.f, pn = have ? peer[buf][lane][2] : 0.f;
+          total = warp_sum(ps);
+          const float d = pn > 0.f ? ps / pn - total * inv_n : 0.f;
+          sq = warp_sum(fmaf(pn * d, d, pq));
+        }
+        s[r] = total;
+        m2[r] = sq;
       }
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r) mean[r] = s[r] * inv_n;
     float rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       rstd[r] = 1.f / sqrtf(m2[r] * inv_n + p.eps);
-      if (at.t == 0 && row + r * step < rows) {
+      if (at.t == 0 && at.rank == 0 && row + r * step < rows) {
         p.mean[row + r * step] = mean[r];
         p.rstd[row + r * step] = rstd[r];
       }
@@ -212,6 +242,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     }
     out += R * out_step;
   }
+  if (CLUSTER) cluster_barrier();      // no CTA leaves while a peer may still write into it
 }
 
 // ---- long rows ---------------------------------------------------------------------------------
@@ -223,7 +254,7 @@ __global__ void __launch_bounds__(kMaxTeam, 2) ln_fwd_long(LnArgs p, RowPlan q) 
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxTeam / 32];
   __shared__ float counts[kMaxTeam / 32];
-  __shared__ float peer[2][8][3];
+  __shared__ float peer[2][kMaxCluster][3];
   constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1;
   constexpr uint32_t kAll = (1u << E) - 1;
   if (q.cluster > 1) cluster_barrier();      // every CTA has started before one writes into another
@@ -242,13 +273,14 @@ __global__ void __launch_bounds__(kMaxTeam, 2) ln_fwd_long(LnArgs p, RowPlan q) 
   count = warp_sum(count);
   if (lane == 0) counts[warp] = count;
 
+  const int ends = last_rows<T, EDGE>(rows, p.cols);
   auto fetch = [&](int row, int k) {
     if (row >= rows || !mask_of(k)) return;
     const size_t a = row_offset<T, EDGE>(row, p.ld_a, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
-    ring_copy<EDGE>(slots + (k * kOps) * kUnit, p.a, a, p.rows * p.cols * sizeof(T));
+    ring_copy(slots + (k * kOps) * kUnit, p.a, a, EDGE && row >= ends, p.rows * p.cols * sizeof(T));
     if (RES) {
       const size_t b = row_offset<T, EDGE>(row, p.ld_b, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
-      ring_copy<EDGE>(slots + (k * kOps + 1) * kUnit, p.b, b, p.rows * p.cols * sizeof(T));
+      ring_copy(slots + (k * kOps + 1) * kUnit, p.b, b, EDGE && row >= ends, p.rows * p.cols * sizeof(T));
     }
   };
   // with a residual the sum is kept as fp32 in the granule's two slots
@@ -393,14 +425,14 @@ int launch_fwd(Kernel kernel, std::atomic<int>* cache, const LnArgs& p, RowPlan 
   int regs = 0;
   if (int rc = prepare("layer_norm_fwd", kernel, cache, &regs)) return rc;
   size_grid(p.rows, resident(q.groups * q.team, regs, q.smem), &q);
-  fit_clusters(kernel, &q);
+  if (!fit_clusters(kernel, &q)) return kDoesNotFit;
   return launch_rows("layer_norm_fwd", kernel, q, st, p, q);
 }
 
-template <typename T, int K, bool RES, bool EDGE>
+template <typename T, int K, bool RES, bool EDGE, bool CLUSTER>
 int rows_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
   static std::atomic<int> cache[64];
-  return launch_fwd(ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE>, cache, p, q, st);
+  return launch_fwd(ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE, CLUSTER>, cache, p, q, st);
 }
 
 template <typename T, bool RES, bool EDGE>
@@ -411,11 +443,13 @@ int long_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
 
 template <typename T, bool RES, bool EDGE>
 int pick_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
+  if (q.cluster > 1)
+    return q.per_thread * kE<T> == 16 ? rows_fwd<T, 16 / kE<T>, RES, EDGE, true>(p, q, st) : rows_fwd<T, 32 / kE<T>, RES, EDGE, true>(p, q, st);
   switch (q.per_thread) {
-    case 1: return rows_fwd<T, 1, RES, EDGE>(p, q, st);
-    case 2: return rows_fwd<T, 2, RES, EDGE>(p, q, st);
-    case 4: return rows_fwd<T, 4, RES, EDGE>(p, q, st);
-    default: return rows_fwd<T, 32 / kE<T>, RES, EDGE>(p, q, st);
+    case 1: return rows_fwd<T, 1, RES, EDGE, false>(p, q, st);
+    case 2: return rows_fwd<T, 2, RES, EDGE, false>(p, q, st);
+    case 4: return rows_fwd<T, 4, RES, EDGE, false>(p, q, st);
+    default: return rows_fwd<T, 32 / kE<T>, RES, EDGE, false>(p, q, st);
   }
 }
 
@@ -424,14 +458,16 @@ int fwd(const LnArgs& p, bool granules, cudaStream_t st) {
   RowPlan q;
   const int ops = p.b ? 2 : 1;
   const bool edge = p.cols % kE<T> != 0;
+  int rc = kDoesNotFit;
   if (granules && plan_fwd_rows(p.rows, p.cols, sizeof(T), ops, &q)) {
-    if (p.b) return edge ? pick_fwd<T, true, true>(p, q, st) : pick_fwd<T, true, false>(p, q, st);
-    return edge ? pick_fwd<T, false, true>(p, q, st) : pick_fwd<T, false, false>(p, q, st);
+    if (p.b) rc = edge ? pick_fwd<T, true, true>(p, q, st) : pick_fwd<T, true, false>(p, q, st);
+    else rc = edge ? pick_fwd<T, false, true>(p, q, st) : pick_fwd<T, false, false>(p, q, st);
   }
-  if (granules && plan_fwd_long(p.rows, p.cols, sizeof(T), ops, &q)) {
-    if (p.b) return edge ? long_fwd<T, true, true>(p, q, st) : long_fwd<T, true, false>(p, q, st);
-    return edge ? long_fwd<T, false, true>(p, q, st) : long_fwd<T, false, false>(p, q, st);
+  if (rc == kDoesNotFit && granules && plan_fwd_long(p.rows, p.cols, sizeof(T), ops, &q)) {
+    if (p.b) rc = edge ? long_fwd<T, true, true>(p, q, st) : long_fwd<T, true, false>(p, q, st);
+    else rc = edge ? long_fwd<T, false, true>(p, q, st) : long_fwd<T, false, false>(p, q, st);
   }
+  if (rc != kDoesNotFit) return rc;
   ln_fwd_any<T><<<grid_for(p.rows, 1, 8), kBlock, 0, st>>>(p);
   return after_launch("layer_norm_fwd");
 }

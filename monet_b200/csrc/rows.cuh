@@ -24,7 +24,8 @@ namespace mb {
 
 // Threads of a CTA: what the registers of an SM hold at 80 a thread, or 128 where a thread has 32 values.
 constexpr int kMaxThreads = 768, kMaxThreadsWide = 512;
-constexpr int kMaxTeam = 512;     // threads of a CTA that share a row
+constexpr int kMaxTeam = 512;     // threads of a CTA that share a row (a CTA of a cluster: all of them)
+constexpr int kMaxCluster = 16;
 constexpr int kUnit = 512;
 template <typename T> constexpr int kE = 16 / static_cast<int>(sizeof(T));    // elements of a granule
 template <typename T> constexpr int kPairs = kE<T> / 2;
@@ -101,12 +102,17 @@ __device__ __forceinline__ void cp_async_wait(int n) {
     default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
   }
 }
-// The granule at byte `off` of a tensor of `bytes`.
-template <bool EDGE>
-__device__ __forceinline__ void ring_copy(uint32_t dst, const void* base, size_t off, size_t bytes) {
+// The granule at byte `off` of a tensor; with `last`, one that may reach behind the tensor's end, where
+// it is filled with zeros.
+__device__ __forceinline__ void ring_copy(uint32_t dst, const void* base, size_t off, bool last, size_t bytes) {
   const char* src = static_cast<const char*>(base) + off;
-  if (EDGE) cp_async16(dst, src, bytes - off >= 16 ? 16 : static_cast<int>(bytes - off));   // zeros behind the tensor's end
+  if (last) cp_async16(dst, src, bytes - off >= 16 ? 16 : static_cast<int>(bytes - off));
   else cp_async16(dst, src, 16);
+}
+// Rows from this one on have granules that may reach behind the tensor's end.
+template <typename T, bool EDGE>
+__device__ __forceinline__ int last_rows(int rows, size_t cols) {
+  return EDGE ? rows - 1 - (cols < kE<T> ? kE<T> : 0) : rows;
 }
 
 // ---- pairs of fp32 -------------------------------------------------------------------------
@@ -286,9 +292,31 @@ __device__ __forceinline__ float warp_sums(const float (&s)[4]) {
   for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
+// (sum, squared deviations from the own mean) of `n` values each in N sets of a team's lanes (a power of
+// two up to 32), merged: for equal counts n the deviations grow by (sum a - sum b)^2 / 2n.  One pass
+// over the lanes instead of one for the mean and another for the deviations.
+template <int N>
+__device__ __forceinline__ void merge_lanes(float (&s)[N], float (&m2)[N], int lanes, float n) {
+  float f = 0.5f / n;
+  for (int o = 1; o < lanes; o <<= 1, f *= 0.5f)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float t = __shfl_xor_sync(0xffffffffu, s[i], o), d = s[i] - t;
+      m2[i] = fmaf(d * f, d, m2[i] + __shfl_xor_sync(0xffffffffu, m2[i], o));
+      s[i] += t;
+    }
+}
 // The N values of a row of `n` <= 16 rows of N floats in shared memory summed over the rows, by every lane.
 template <int N>
 __device__ __forceinline__ void gather(const float* f, int n, float (&s)[N]) {
+  if (n <= 8) {        // few: every lane reads them all, without a chain of shuffles
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = f[i];
+    for (int w = 1; w < n; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] += f[w * N + i];
+    return;
+  }
   const int lane = threadIdx.x & 31;
   float x = lane < N * n ? f[lane] : 0.f;
   if (N * 16 > 32 && N * n > 32) x += lane + 32 < N * n ? f[lane + 32] : 0.f;
