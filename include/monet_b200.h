@@ -412,12 +412,15 @@ typedef struct {
  * dense; so may `sum` (not the one that y aliases).  ld_a: x, ld_b: residual.                */
 int mb_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias,
                       void* y, void* sum, float* mean, float* rstd, const mb_ln_desc* d,
-                      const mb_dropout_desc* drop, void* stream);
-/* Bytes of scratch mb_layer_norm_bwd needs.                                                 */
-size_t mb_layer_norm_workspace_bytes(const mb_ln_desc* d);
+                      const mb_dropout_desc* drop, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* Bytes of scratch the two entries need (forward: 0 unless rows are long; then 4-byte, backward
+ * 16-byte aligned).                                                                         */
+size_t mb_layer_norm_fwd_workspace_bytes(const mb_ln_desc* d);
+size_t mb_layer_norm_bwd_workspace_bytes(const mb_ln_desc* d);
 /* Backward of the above.  `kept` is v (kept_is_output = 0: xhat = (v - mean) * rstd) or the output
- * y (1: xhat = (y - bias) / weight; needs no mean; a weight of zero is undefined, as for batch norm,
- * and gives NaN).  With g = dy * weight:
+ * y (1: xhat = (y - bias) / weight; needs no mean; a weight of zero is undefined, as for batch norm:
+ * NaN or infinite gradients in its column).  With g = dy * weight:
  *   dv = rstd * (g - mean(g) - xhat * mean(g * xhat)) (+ dsum, the gradient of `sum`, if given),
  *   dweight = sum over rows of dy * xhat, dbias = sum over rows of dy  (either may be NULL).
  * dv goes to `dv`; dropout(dv), the gradient of x, to `dx` when that is non-NULL.  The sums over

@@ -116,8 +116,9 @@ PROTOTYPES = {
     "mb_global_avgpool_fwd": (C.c_int, [c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "mb_global_avgpool_bwd": (C.c_int, [c_f, c_f, C.c_int, C.c_int, C.c_int, C.c_int, c_f]),
     "mb_dropout": (C.c_int, [c_f, c_f, c_sz, C.c_int, C.POINTER(DropoutDesc), c_f]),
-    "mb_layer_norm_fwd": (C.c_int, [c_f] * 8 + [C.POINTER(LnDesc), C.POINTER(DropoutDesc), c_f]),
-    "mb_layer_norm_workspace_bytes": (c_sz, [C.POINTER(LnDesc)]),
+    "mb_layer_norm_fwd": (C.c_int, [c_f] * 8 + [C.POINTER(LnDesc), C.POINTER(DropoutDesc), c_f, c_sz, c_f]),
+    "mb_layer_norm_fwd_workspace_bytes": (c_sz, [C.POINTER(LnDesc)]),
+    "mb_layer_norm_bwd_workspace_bytes": (c_sz, [C.POINTER(LnDesc)]),
     "mb_layer_norm_bwd": (C.c_int, [c_f, c_f, C.c_int] + [c_f] * 9 + [C.POINTER(LnDesc), C.POINTER(DropoutDesc),
                                                                     c_f, c_sz, c_f]),
 }

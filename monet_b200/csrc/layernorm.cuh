@@ -47,9 +47,8 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 
 // ---- which kernel ------------------------------------------------------------------------------
 // Rows whose tensors lie on granule boundaries in the same way are walked in granules (rows.cuh): a
-// thread holds 4 to 32 values, a team up to kMaxTeam threads.  Longer rows: forward stays in the shared
-// memory of up to eight CTAs, backward in the registers of up to eight.  Everything else takes the
-// element-wise kernels.
+// thread holds 4 to 32 values, a team up to kMaxTeam threads, a cluster up to four of these.  Longer rows
+// are walked twice, for the sums and for the result.  Everything else takes the element-wise kernels.
 constexpr size_t kSmemLimit = 225 * 1024;
 
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
@@ -105,8 +104,8 @@ inline bool plan_ring(size_t rows, int r, int ops, int least, size_t params, Row
   if (params >= kSmemLimit) return false;
   const size_t deep = (kSmemLimit - params) / (r * stage);
   if (deep < static_cast<size_t>(least)) return false;
-  const size_t each = (rows + static_cast<size_t>(num_sms()) * q->groups - 1) / (static_cast<size_t>(num_sms()) * q->groups);
-  const size_t of_use = (each + r - 1) / r;                  // no more than a team has rows, if every SM has a CTA
+  const size_t teams = static_cast<size_t>(num_sms() / q->cluster > 0 ? num_sms() / q->cluster : 1) * q->groups;
+  const size_t of_use = ((rows + teams - 1) / teams + r - 1) / r;      // no more than a team has rows, if every SM has a CTA
   int n = 8 / r;
   if (deep < static_cast<size_t>(n)) n = static_cast<int>(deep);
   if (of_use < static_cast<size_t>(n) && q->period == 1) n = static_cast<int>(of_use);
@@ -143,7 +142,7 @@ inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from
     for (teams = q->team <= 32 || teams > fit ? fit : teams; teams >= 1; --teams) {
       plan_groups(rows, teams, q);
       const size_t fold = q->groups > 1 ? static_cast<size_t>((q->groups + 1) / 2) * q->team * q->per_thread * elems * 2 * sizeof(float) : 0;
-      if (fold <= kSmemLimit && plan_ring(rows, r, ops, q->cluster == kMaxCluster ? 1 : 2, params, q)) {
+      if (fold <= kSmemLimit && plan_ring(rows, r, ops, 2, params, q)) {
         if (fold > q->smem) q->smem = fold;                  // the teams' column sums are folded there
         return true;
       }
@@ -159,12 +158,10 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   if (most > static_cast<size_t>(kMaxTeam) * kMaxCluster * (32 / elems)) return false;
   for (q->cluster = 1; q->cluster <= kMaxCluster; q->cluster *= 2) {
     const int chunk = ceil_div(static_cast<long long>(most), q->cluster);
-    int values = q->cluster > 1 ? 0 : one_warp_values(chunk, elems);
-    if (!values) values = 32;      // (16384 x 8192 bf16: 115 us against 154 with 16)
-    // a cluster's CTA has one team, so it takes as many threads as it can
-    if (q->cluster > 1 && chunk * elems <= 16 * kMaxThreads) values = 16;
+    int values = q->cluster > 1 ? 32 : one_warp_values(chunk, elems);
+    if (!values) values = 32;      // (16384 x 8192 bf16: 107 us against 154 with 16)
     plan_team(chunk, elems, values, q);
-    if (q->team > (values == 16 && q->cluster > 1 ? kMaxThreads : kMaxTeam)) continue;
+    if (q->team > kMaxTeam) continue;
     const int r = fwd_rows_between_barriers(q->per_thread, elems);
     const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
     for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
@@ -175,23 +172,28 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   return false;
 }
 
-// One row in the shared memory of 1 to 8 CTAs, of which two share an SM if they are small enough.
-inline bool plan_fwd_long(size_t rows, size_t cols, int elem, int ops, RowPlan* q) {
+// Long rows: `cluster` chunks of up to kMaxThreads threads with 16 values each, as many as use the SMs
+// best.  `params` fp32 values of each column lie beside the ring.
+inline bool plan_long(size_t rows, size_t cols, int elem, int ops, int params, RowPlan* q) {
   if (rows >> 30) return false;
-  const size_t most = row_granules(cols, 16 / elem, &q->period);
-  for (size_t limit = 106 * 1024; limit <= kSmemLimit; limit += kSmemLimit - 106 * 1024)
-    for (q->cluster = 1; q->cluster <= 8; q->cluster *= 2) {
-      const size_t chunk = (most + q->cluster - 1) / q->cluster;
-      if (chunk > 65536) continue;
-      q->chunk = static_cast<int>(chunk);
-      q->team = kMaxTeam;
-      q->groups = 1;
-      q->stages = 1;
-      q->per_thread = ceil_div(q->chunk, q->team);
-      q->smem = static_cast<size_t>(q->team) / 32 * q->per_thread * ops * kUnit;
-      if (q->smem <= limit) return true;
+  const int elems = 16 / elem, sms = num_sms();
+  const size_t most = row_granules(cols, elems, &q->period);
+  q->per_thread = 16 / elems;
+  q->groups = 1;
+  const int least = ceil_div(static_cast<long long>(most), static_cast<long long>(kMaxThreads) * q->per_thread);
+  double best = 0.0;
+  for (int n = least; n <= 2 * least; ++n) {
+    const int unit = n * q->period, rounds = ceil_div(unit, sms);
+    const double use = unit <= sms ? static_cast<double>(sms / unit * unit) / sms : static_cast<double>(unit) / (rounds * sms);
+    if (use > best + 0.02) {
+      best = use;
+      q->cluster = n;
     }
-  return false;
+  }
+  q->chunk = ceil_div(static_cast<long long>(most), q->cluster);
+  q->team = ceil_div(q->chunk, 32 * q->per_thread) * 32;
+  if (q->team < 64) q->team = 64;                            // (a long row has far more)
+  return plan_ring(rows, 1, ops, 1, static_cast<size_t>(q->team) * q->per_thread * elems * 4 * params, q);
 }
 
 // CTAs: `per_sm` on every SM, no more than there are rows, a whole number of clusters of each residue.
@@ -216,7 +218,6 @@ int prepare(const char* who, Kernel kernel, std::atomic<int>* cache, int* regs) 
   if (r == 0) {
     cudaFuncAttributes a;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return fail(MB_ERR_LAUNCH, "%s: %s", who, cudaGetErrorString(cudaGetLastError()));
     r = a.numRegs + 1;
@@ -235,8 +236,20 @@ inline int resident(int threads, int regs, size_t smem) {
   return k < 1 ? 1 : k > 16 ? 16 : k;
 }
 
+// Launched while the kernel before it in the stream still runs; it waits for that one's end by itself
+// (griddepcontrol.wait) before it touches memory.
 template <typename... KArgs, typename... Args>
-int launch_rows(const char* who, void (*kernel)(KArgs...), const RowPlan& q, cudaStream_t st, Args... args) {
+void launch_dependent(cudaLaunchConfig_t* cfg, void (*kernel)(KArgs...), Args... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+  cudaLaunchKernelEx(cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+template <typename... KArgs, typename... Args>
+int launch_rows(const char* who, int pass, void (*kernel)(KArgs...), const RowPlan& q, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(q.grid);
   cfg.blockDim = dim3(q.groups * q.team);
@@ -247,8 +260,9 @@ int launch_rows(const char* who, void (*kernel)(KArgs...), const RowPlan& q, cud
   attr[0].val.clusterDim.x = q.cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = q.cluster > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+  cfg.numAttrs = pass == kCluster ? 1 : 0;
+  if (pass == kApply) launch_dependent(&cfg, kernel, args...);
+  else cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
   return after_launch(who);
 }
 

@@ -4,7 +4,7 @@
 namespace mb {
 namespace {
 
-// Backward.  partial[team CTA][0][col] = sum of dy xhat, [1][col] = sum of dy over the CTA's rows.
+// Backward.  partial[CTA of a row][0][col] = sum of dy xhat, [1][col] = sum of dy over the CTA's rows.
 //
 // R rows are handled between two barriers: their sums are formed from a first reading of the
 // ring, then the rows are read a second time to form dv.  Reading twice costs shared-memory loads but
@@ -12,18 +12,23 @@ namespace {
 // (in registers where a thread has one granule).  With 80 registers a thread, 24 warps share an SM,
 // and one team computes while another waits for its barrier.
 //
+// Long rows (PASS): kStats writes the two sums of each chunk, sums_of_rows[row][chunk][2]; kApply finds
+// the rows' sums there, [row][2], and forms dv and the column sums in one reading.
+//
 // With t = v - mean or y - b:  sum g xhat = rstd sum (dy t) w  or  sum dy t  (the weight cancels), and
 // dw = sum over rows of (dy t) rstd  or  (sum dy t) / w, so xhat itself is never formed.
-template <typename T, int K, int R, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial) {
+template <typename T, int K, int R, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, int PASS>
+__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_bwd_rows(LnArgs p, RowPlan q, float* partial, float* sums_of_rows) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float red[2][kMaxThreads / 32][2 * R];      // double-buffered by row: one barrier a row
   __shared__ float peer[2][kMaxCluster][2 * R];
-  if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
-  constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 2 : 1;
+  if (PASS == kCluster) cluster_barrier();      // every CTA has started before one writes into another
+  if (PASS == kApply) asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int E = kE<T>, P = kPairs<T>, kOps = DSUM && PASS != kStats ? 3 : 2, kSlots = K * kOps, kKinds = FROM_Y ? 2 : 1;
   constexpr int kParam = kParamUnits<T> * kUnit;
   constexpr bool kInRegs = K == 1;
-  const RowWalk at(q, p.cols, E);
+  // the result's pass walks the rows backwards: the last ones are still in L2
+  const RowWalk at(q, p.cols, E, PASS == kApply ? static_cast<int>(p.rows) - 1 : -1);
   const float inv_n = 1.f / static_cast<float>(p.cols);
   const int j0 = at.rank * q.chunk + at.t;           // the thread's granules: j0 + k * team
   const int rows = static_cast<int>(p.rows), step = at.step;
@@ -42,15 +47,16 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   }
 
   // byte offset of the thread's first granule in the first of the rows at hand (all tensors are dense)
-  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, j0) * sizeof(T);
-  const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
+  auto actual = [&](int i) { return PASS == kApply ? rows - 1 - i : i; };
+  size_t out = row_offset<T, EDGE>(at.first < rows ? actual(at.first) : 0, p.cols, p.cols, j0) * sizeof(T);
+  const size_t out_step = (PASS == kApply ? ~size_t(0) : 1) * step * p.cols * sizeof(T);
   const int ends = last_rows<T, EDGE>(rows, p.cols);
   auto fetch = [&](uint32_t stage, int i, size_t off) {
 #pragma unroll
     for (int o = 0; o < kOps; ++o)
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (mask[k]) ring_copy(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, EDGE && i >= ends, p.rows * p.cols * sizeof(T));
+        if (mask[k]) ring_copy(stage + (k * kOps + o) * kUnit, o == 0 ? p.a : o == 1 ? p.b : p.c, off + k * kstep, EDGE && actual(i) >= ends, p.rows * p.cols * sizeof(T));
   };
 
   float2 wr[P], nbr[P];                // kInRegs: the weight; with FROM_Y minus the bias
@@ -73,6 +79,10 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     }
   };
 
+  auto column_sums = [&](int k, int i, float2 u, float2 dy, float rstd) {      // u = dy t
+    ab[k][i] = add2(ab[k][i], dy);
+    aw[k][i] = FROM_Y ? add2(aw[k][i], u) : fma2(u, both(rstd), aw[k][i]);
+  };
   // slots that are never fetched hold zeros, so that the sums need not ask
 #pragma unroll
   for (int k = 0; k < K; ++k)
@@ -110,8 +120,8 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = first + r * step;
-      m[r] = !FROM_Y && i < rows ? __ldg(p.mean + i) : 0.f;
-      s[r] = i < rows ? __ldg(p.rstd + i) : 0.f;
+      m[r] = !FROM_Y && i < rows ? __ldg(p.mean + actual(i)) : 0.f;
+      s[r] = i < rows ? __ldg(p.rstd + actual(i)) : 0.f;
     }
   };
   statistics(row, mean, rstd);
@@ -121,6 +131,8 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     float mean_next[R], rstd_next[R];
     statistics(row + R * step, mean_next, rstd_next);
     cp_async_wait(q.stages / R - 1);
+    float s[2 * R];                      // sum dy w and sum g t of each row
+    if constexpr (PASS != kApply) {
     float2 t1[R], t2[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) t1[r] = t2[r] = both(0.f);
@@ -137,18 +149,11 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         for (int i = 0; i < P; ++i) {
           const float2 u = mul2(dy[i], t[i]);
           t1[r] = fma2(dy[i], w[i], t1[r]);
-          ab[k][i] = add2(ab[k][i], dy[i]);
-          if (FROM_Y) {
-            t2[r] = add2(t2[r], u);
-            aw[k][i] = add2(aw[k][i], u);
-          } else {
-            t2[r] = fma2(u, w[i], t2[r]);
-            aw[k][i] = fma2(u, both(rstd[r]), aw[k][i]);
-          }
+          t2[r] = FROM_Y ? add2(t2[r], u) : fma2(u, w[i], t2[r]);
+          if (PASS != kStats) column_sums(k, i, u, dy[i], rstd[r]);
         }
       }
     }
-    float s[2 * R];                      // sum dy w and sum g t of each row
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       s[2 * r] = t1[r].x + t1[r].y;
@@ -161,7 +166,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
       if ((threadIdx.x & (16 / R - 1)) == 0) red[buf][threadIdx.x >> 5][(threadIdx.x & 31) / (16 / R)] = x;
       team_barrier(at.group, q.team);
       gather(red[buf][at.group * (q.team >> 5)], q.team >> 5, s);
-      if (CLUSTER) {
+      if (PASS == kCluster) {
         if (threadIdx.x < q.cluster)
 #pragma unroll
           for (int i = 0; i < 2 * R; ++i) put_remote(&peer[buf][at.rank][i], threadIdx.x, s[i]);
@@ -169,6 +174,25 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         gather(peer[buf][0], q.cluster, s);
       }
     }
+      if constexpr (PASS == kStats) {
+        if (threadIdx.x == 0)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (row + r * step < rows) {
+              float* to = sums_of_rows + (static_cast<size_t>(row + r * step) * q.cluster + at.rank) * 2;
+              to[0] = s[2 * r];
+              to[1] = s[2 * r + 1];
+            }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int i = row + r * step;
+        s[2 * r] = i < rows ? __ldg(sums_of_rows + 2 * static_cast<size_t>(actual(i))) : 0.f;
+        s[2 * r + 1] = i < rows ? __ldg(sums_of_rows + 2 * static_cast<size_t>(actual(i)) + 1) : 0.f;
+      }
+    }
+    if constexpr (PASS != kStats) {
     uint32_t gone[R][K];                 // what dropout drops, the pairs' sign bits folded into a word
     if (DROP) {
       const unsigned long long key = __ldg(p.drop.seed);
@@ -198,6 +222,9 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         const float2 c1 = both(-s[2 * r] * inv_n), c2 = both(FROM_Y ? -s[2 * r + 1] * inv_n : -s[2 * r + 1] * inv_n * rstd[r] * rstd[r]);
         float2 t[P], d[P];
         read(stage + r * stride, k, mean[r], t, d);
+        if (PASS == kApply)
+#pragma unroll
+          for (int i = 0; i < P; ++i) column_sums(k, i, mul2(d[i], t[i]), d[i], rstd[r]);
 #pragma unroll
         for (int i = 0; i < P; ++i) d[i] = fma2(d[i], w[i], c1);
         if (FROM_Y) {
@@ -225,6 +252,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         }
       }
     }
+    }
     // the next rows into the slots just read for the last time
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -239,8 +267,8 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
       rstd[r] = rstd_next[r];
     }
   }
-  if (CLUSTER) cluster_barrier();      // no CTA leaves while a peer may still write into it
-  if (!partial) return;
+  if (PASS == kCluster) cluster_barrier();      // no CTA leaves while a peer may still write into it
+  if (PASS == kStats || !partial) return;
   if (FROM_Y) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -299,6 +327,25 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
           }
       }
     }
+  }
+}
+
+// The sums of a long row from those of its chunks: a warp a row, into [row][2].
+__global__ void __launch_bounds__(kBlock) ln_bwd_combine(const float* chunk_sums, int chunks, size_t rows, float* row_sums) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const size_t row = static_cast<size_t>(blockIdx.x) * (kBlock / 32) + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  float a = 0.f, b = 0.f;
+  for (int i = lane; i < chunks; i += 32) {
+    a += chunk_sums[(row * chunks + i) * 2];
+    b += chunk_sums[(row * chunks + i) * 2 + 1];
+  }
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if (lane == 0) {
+    row_sums[2 * row] = a;
+    row_sums[2 * row + 1] = b;
   }
 }
 
@@ -405,12 +452,7 @@ int finish(const float* partial, int parts, size_t cols, void* dw, void* db, boo
   cfg.gridDim = dim3(static_cast<unsigned>((cols + 31) / 32));
   cfg.blockDim = dim3(32, 32);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, ln_bwd_finish<T>, partial, parts, cols, dw, db, w_f32);
+  launch_dependent(&cfg, ln_bwd_finish<T>, partial, parts, cols, dw, db, w_f32);
   return after_launch("layer_norm_bwd_finish");
 }
 
@@ -429,45 +471,69 @@ bool plan_bwd(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
   return true;
 }
 
+bool plan_bwd_long(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
+  if (!plan_long(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, from_y ? 2 : 1, q)) return false;
+  size_grid(d->rows, 1, q);
+  return true;
+}
+
 struct Grads { void *dw, *db; float* ws; };
 
-template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, bool CLUSTER>
-int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st) {
+// Scratch: the partial column sums; for long rows also the chunks' and the rows' sums.
+template <typename T, int K, bool FROM_Y, bool DSUM, bool DROP, bool EDGE, int PASS>
+int launch_bwd(const LnArgs& p, RowPlan q, const Grads& g, cudaStream_t st, float* sums_of_rows = nullptr) {
   static std::atomic<int> cache[64];
-  auto kernel = ln_bwd_rows<T, K, bwd_rows_between_barriers(K), FROM_Y, DSUM, DROP, EDGE, CLUSTER>;
+  auto kernel = ln_bwd_rows<T, K, bwd_rows_between_barriers(K), FROM_Y, DSUM, DROP, EDGE, PASS>;
   int regs = 0;
   if (int rc = prepare("layer_norm_bwd", kernel, cache, &regs)) return rc;
-  if (!fit_clusters(kernel, &q)) return kDoesNotFit;
-  const bool sums = g.dw || g.db;
-  if (int rc = launch_rows("layer_norm_bwd", kernel, q, st, p, q, sums ? g.ws : nullptr)) return rc;
+  if (PASS == kCluster && !fit_clusters(kernel, &q)) return kDoesNotFit;
+  const bool sums = PASS != kStats && (g.dw || g.db);
+  if (int rc = launch_rows("layer_norm_bwd", PASS, kernel, q, st, p, q, sums ? g.ws : nullptr, sums_of_rows)) return rc;
   return sums ? finish<T>(g.ws, q.grid / q.cluster, p.cols, g.dw, g.db, p.w_f32, st) : MB_OK;
 }
 
 template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
 int pick_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
   constexpr int most = 32 / kE<T>;
-  if (q.cluster > 1) return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, true>(p, q, g, st);
+  if (q.cluster > 1) return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, kCluster>(p, q, g, st);
   switch (q.per_thread) {
-    case 1: return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-    case 2: return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-    case 4: return launch_bwd<T, 4, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
-    default: return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, false>(p, q, g, st);
+    case 1: return launch_bwd<T, 1, FROM_Y, DSUM, DROP, EDGE, kWhole>(p, q, g, st);
+    case 2: return launch_bwd<T, 2, FROM_Y, DSUM, DROP, EDGE, kWhole>(p, q, g, st);
+    case 4: return launch_bwd<T, 4, FROM_Y, DSUM, DROP, EDGE, kWhole>(p, q, g, st);
+    default: return launch_bwd<T, most, FROM_Y, DSUM, DROP, EDGE, kWhole>(p, q, g, st);
   }
 }
 
+template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
+int long_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
+  constexpr int K = 16 / kE<T>;
+  float* row_sums = g.ws + static_cast<size_t>(q.grid / q.cluster) * 2 * p.cols;
+  float* chunk_sums = row_sums + 2 * p.rows;
+  if (int rc = launch_bwd<T, K, FROM_Y, false, false, EDGE, kStats>(p, q, g, st, chunk_sums)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + kBlock / 32 - 1) / (kBlock / 32)));
+  cfg.blockDim = dim3(kBlock);
+  cfg.stream = st;
+  launch_dependent(&cfg, ln_bwd_combine, static_cast<const float*>(chunk_sums), q.cluster, p.rows, row_sums);
+  if (int rc = after_launch("layer_norm_bwd_combine")) return rc;
+  return launch_bwd<T, K, FROM_Y, DSUM, DROP, EDGE, kApply>(p, q, g, st, row_sums);
+}
+
 template <typename T, bool FROM_Y, bool DSUM, bool DROP>
-int pick_edge(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
+int pick_edge(const LnArgs& p, const RowPlan& q, bool is_long, const Grads& g, cudaStream_t st) {
+  if (is_long) return p.cols % kE<T> ? long_bwd<T, FROM_Y, DSUM, DROP, true>(p, q, g, st) : long_bwd<T, FROM_Y, DSUM, DROP, false>(p, q, g, st);
   return p.cols % kE<T> ? pick_bwd<T, FROM_Y, DSUM, DROP, true>(p, q, g, st) : pick_bwd<T, FROM_Y, DSUM, DROP, false>(p, q, g, st);
 }
 
 template <typename T, bool FROM_Y>
 int bwd(const LnArgs& p, const mb_ln_desc* d, bool granules, const Grads& g, cudaStream_t st) {
-  RowPlan q;
   // (a dx that equals dv because nothing is dropped is rare enough for the element-wise kernels)
-  if (granules && (p.drop.on || !p.out2) && plan_bwd(d, p.c ? 3 : 2, FROM_Y, &q)) {
+  for (int is_long = 0; is_long <= 1 && granules && (p.drop.on || !p.out2); ++is_long) {
+    RowPlan q;
+    if (is_long ? !plan_bwd_long(d, p.c ? 3 : 2, FROM_Y, &q) : !plan_bwd(d, p.c ? 3 : 2, FROM_Y, &q)) continue;
     int rc;
-    if (p.drop.on) rc = p.c ? pick_edge<T, FROM_Y, true, true>(p, q, g, st) : pick_edge<T, FROM_Y, false, true>(p, q, g, st);
-    else rc = p.c ? pick_edge<T, FROM_Y, true, false>(p, q, g, st) : pick_edge<T, FROM_Y, false, false>(p, q, g, st);
+    if (p.drop.on) rc = p.c ? pick_edge<T, FROM_Y, true, true>(p, q, is_long, g, st) : pick_edge<T, FROM_Y, false, true>(p, q, is_long, g, st);
+    else rc = p.c ? pick_edge<T, FROM_Y, true, false>(p, q, is_long, g, st) : pick_edge<T, FROM_Y, false, false>(p, q, is_long, g, st);
     if (rc != kDoesNotFit) return rc;
   }
   if (g.dw || g.db) {      // before the outputs, which may lie over the inputs
@@ -487,14 +553,21 @@ using namespace mb;
 
 extern "C" {
 
-size_t mb_layer_norm_workspace_bytes(const mb_ln_desc* d) {
-  if (!d || d->cols == 0 || d->rows == 0 || !dtype_bytes(d->dtype)) return 0;
+size_t mb_layer_norm_bwd_workspace_bytes(const mb_ln_desc* d) {
+  if (!d || d->cols == 0 || d->cols > 0x7fffffffULL || d->rows == 0 || !dtype_bytes(d->dtype)) return 0;
   // which kernel runs also depends on addresses: enough for any
-  int parts = column_parts(d);
-  RowPlan q;
-  for (int form = 0; form < 4; ++form)
-    if (plan_bwd(d, 2 + form / 2, form % 2, &q) && q.grid / q.cluster > parts) parts = q.grid / q.cluster;
-  return static_cast<size_t>(parts) * 2 * d->cols * sizeof(float);
+  size_t floats = static_cast<size_t>(column_parts(d)) * 2 * d->cols;
+  for (int form = 0; form < 4; ++form) {
+    RowPlan q;
+    size_t n = 0;
+    const bool fits = plan_bwd(d, 2 + form / 2, form % 2, &q);
+    if (fits) n = static_cast<size_t>(q.grid / q.cluster) * 2 * d->cols;
+    if (n > floats) floats = n;
+    if ((!fits || q.cluster > 1) && plan_bwd_long(d, 2 + form / 2, form % 2, &q))
+      n = static_cast<size_t>(q.grid / q.cluster) * 2 * d->cols + 2 * d->rows * (1 + static_cast<size_t>(q.cluster));
+    if (n > floats) floats = n;
+  }
+  return floats * sizeof(float);
 }
 
 int mb_layer_norm_bwd(const void* dy, const void* kept, int kept_is_output, const void* dsum, const void* weight,
@@ -519,7 +592,7 @@ int mb_layer_norm_bwd(const void* dy, const void* kept, int kept_is_output, cons
   if (drop && !dx) return fail(MB_ERR_INVALID_ARGUMENT, "%s: dropout needs dx", who);
   if (!natural(d, dy) || !natural(d, kept) || !natural(d, dsum) || !natural(d, dv) || !natural(d, dx) || !aligned(mean, 4) || !aligned(rstd, 4))
     return fail(MB_ERR_INVALID_ARGUMENT, "%s: misaligned pointer", who);
-  if ((dweight || dbias) && (!workspace || !aligned(workspace, 16) || workspace_bytes < mb_layer_norm_workspace_bytes(d)))
+  if (!workspace || !aligned(workspace, 16) || workspace_bytes < mb_layer_norm_bwd_workspace_bytes(d))
     return fail(MB_ERR_WORKSPACE, "%s: workspace too small or misaligned", who);
   const Grads g{dweight, dbias, static_cast<float*>(workspace)};
   const bool granules = d->ld_a == d->cols && d->ld_b == d->cols && (!dsum || d->ld_c == d->cols) &&

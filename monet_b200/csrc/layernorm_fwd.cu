@@ -25,20 +25,25 @@ __device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, u
   return sum;
 }
 
-template <typename T, int K, int R, bool RES, bool EDGE, bool CLUSTER>
-__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q) {
+template <typename T, int K, int R, bool RES, bool EDGE, int PASS>
+__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
   __shared__ float counts[kMaxThreads / 32];
   __shared__ float peer[2][kMaxCluster][3];
-  if (CLUSTER) cluster_barrier();      // every CTA has started before one writes into another
+  if (PASS == kCluster) cluster_barrier();      // every CTA has started before one writes into another
+  if (PASS == kApply) asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1, kSlots = K * kOps;
   constexpr int kParam = kParamUnits<T> * kUnit;
   constexpr uint32_t kAll = (1u << E) - 1;
   constexpr bool kInRegs = K == 1;
-  const RowWalk at(q, p.cols, E);
+  // the result's pass walks the rows backwards: the last ones are still in L2
+  const RowWalk at(q, p.cols, E, PASS == kApply ? static_cast<int>(p.rows) - 1 : -1);
   const float inv_n = 1.f / static_cast<float>(p.cols);
   const int rows = static_cast<int>(p.rows), step = at.step, lane = threadIdx.x & 31, warps = q.team >> 5;
+  auto actual = [&](int i) { return PASS == kApply ? rows - 1 - i : i; };
+  const size_t forth = PASS == kApply ? ~size_t(0) : 1;      // -1 or 1
+  const int begin = at.first < rows ? actual(at.first) : 0;
   const unsigned long long key = RES && p.drop.on ? __ldg(p.drop.seed) : 0;
   const uint32_t stride = (blockDim.x >> 5) * (kSlots * kUnit);
   const uint32_t slots = sm100::smem_u32(ring) + (threadIdx.x >> 5) * (kSlots * kUnit) + lane * 16;
@@ -59,10 +64,10 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     if (lane == 0) counts[threadIdx.x >> 5] = count;
   }
 
-  size_t out = row_offset<T, EDGE>(at.first, p.cols, p.cols, j0) * sizeof(T);
-  const size_t out_step = static_cast<size_t>(step) * p.cols * sizeof(T);
+  size_t out = row_offset<T, EDGE>(begin, p.cols, p.cols, j0) * sizeof(T);
+  const size_t out_step = forth * step * p.cols * sizeof(T);
   // inputs may have gaps between their rows
-  size_t in_a = row_offset<T, EDGE>(at.first, p.ld_a, p.cols, j0) * sizeof(T), in_b = RES ? row_offset<T, EDGE>(at.first, p.ld_b, p.cols, j0) * sizeof(T) : 0;
+  size_t in_a = row_offset<T, EDGE>(begin, p.ld_a, p.cols, j0) * sizeof(T), in_b = RES ? row_offset<T, EDGE>(begin, p.ld_b, p.cols, j0) * sizeof(T) : 0;
   int next = at.first;
   const int ends = last_rows<T, EDGE>(rows, p.cols);
   auto fetch = [&](uint32_t stage) {
@@ -70,11 +75,11 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!mask[k]) continue;
-        ring_copy(stage + (k * kOps) * kUnit, p.a, in_a + k * kstep, EDGE && next >= ends, p.rows * p.cols * sizeof(T));
-        if (RES) ring_copy(stage + (k * kOps + 1) * kUnit, p.b, in_b + k * kstep, EDGE && next >= ends, p.rows * p.cols * sizeof(T));
+        ring_copy(stage + (k * kOps) * kUnit, p.a, in_a + k * kstep, EDGE && actual(next) >= ends, p.rows * p.cols * sizeof(T));
+        if (RES) ring_copy(stage + (k * kOps + 1) * kUnit, p.b, in_b + k * kstep, EDGE && actual(next) >= ends, p.rows * p.cols * sizeof(T));
       }
-      in_a += static_cast<size_t>(step) * p.ld_a * sizeof(T);
-      if (RES) in_b += static_cast<size_t>(step) * p.ld_b * sizeof(T);
+      in_a += forth * step * p.ld_a * sizeof(T);
+      if (RES) in_b += forth * step * p.ld_b * sizeof(T);
     }
     next += step;
   };
@@ -91,7 +96,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   }
 
   float2 wr[P], br[P];
-  if (kInRegs || at.group == 0) {
+  if (PASS != kStats && (kInRegs || at.group == 0)) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
@@ -114,6 +119,18 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   uint32_t stage = slots;
   int row = at.first, buf = 0;
   const int spare = at.spare(q);
+  float mean_next[R], rstd_next[R];
+  auto given = [&](int first) {        // the statistics of the rows from `first` on
+    if constexpr (PASS == kApply) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (first + r * step < rows) {
+          mean_next[r] = __ldg(p.mean + actual(first + r * step));
+          rstd_next[r] = __ldg(p.rstd + actual(first + r * step));
+        }
+    }
+  };
+  given(row);
   for (; row - spare < rows; row += R * step, buf ^= 1) {
     cp_async_wait(q.stages / R - 1);
     float2 v[R][K][P];
@@ -151,6 +168,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
     if (stage >= slots + q.stages * stride) stage = slots;
 
     float mean[R], m2[R];
+    if constexpr (PASS != kApply) {
     auto spread = [&](const float (&centre)[R], bool whole) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -193,7 +211,7 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
           const float d = mine.x * part_inv - total * part_each;
           sq = warp_sum(part_inv > 0.f ? fmaf(part_count * d, d, mine.y) : 0.f);
         }
-        if (CLUSTER) {
+        if (PASS == kCluster) {
           if (threadIdx.x < q.cluster) {
             put_remote(&peer[buf][at.rank][0], threadIdx.x, total);
             put_remote(&peer[buf][at.rank][1], threadIdx.x, sq);
@@ -206,21 +224,35 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
           const float d = pn > 0.f ? ps / pn - total * inv_n : 0.f;
           sq = warp_sum(fmaf(pn * d, d, pq));
         }
+        if (PASS == kStats && threadIdx.x == 0 && row + r * step < rows) {
+          float* to = partial + (static_cast<size_t>(row + r * step) * q.cluster + at.rank) * 3;
+          to[0] = total;
+          to[1] = sq;
+          to[2] = n;
+        }
         s[r] = total;
         m2[r] = sq;
       }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) mean[r] = s[r] * inv_n;
+    }
+    if constexpr (PASS != kStats) {
     float rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      rstd[r] = 1.f / sqrtf(m2[r] * inv_n + p.eps);
-      if (at.t == 0 && at.rank == 0 && row + r * step < rows) {
-        p.mean[row + r * step] = mean[r];
-        p.rstd[row + r * step] = rstd[r];
+      if constexpr (PASS == kApply) {
+        mean[r] = mean_next[r];
+        rstd[r] = rstd_next[r];
+      } else {
+        rstd[r] = 1.f / sqrtf(m2[r] * inv_n + p.eps);
+        if (at.t == 0 && at.rank == 0 && row + r * step < rows) {
+          p.mean[row + r * step] = mean[r];
+          p.rstd[row + r * step] = rstd[r];
+        }
       }
     }
+    given(row + R * step);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float2 w[P], b[P];
@@ -240,146 +272,31 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), v[r][k], mask[k]);
       }
     }
+    }
     out += R * out_step;
   }
-  if (CLUSTER) cluster_barrier();      // no CTA leaves while a peer may still write into it
+  if (PASS == kCluster) cluster_barrier();      // no CTA leaves while a peer may still write into it
 }
 
-// ---- long rows ---------------------------------------------------------------------------------
-// A row lies in the shared memory of up to eight CTAs: it is read from HBM once and walked three
-// times there (sum, deviations, result).  Each granule's slot takes the next row's as soon as the
-// result is written, so that row arrives while this one is stored.
-template <typename T, bool RES, bool EDGE>
-__global__ void __launch_bounds__(kMaxTeam, 2) ln_fwd_long(LnArgs p, RowPlan q) {
-  extern __shared__ __align__(128) uint4 ring[];
-  __shared__ float2 red[2][kMaxTeam / 32];
-  __shared__ float counts[kMaxTeam / 32];
-  __shared__ float peer[2][kMaxCluster][3];
-  constexpr int E = kE<T>, P = kPairs<T>, kOps = RES ? 2 : 1;
-  constexpr uint32_t kAll = (1u << E) - 1;
-  if (q.cluster > 1) cluster_barrier();      // every CTA has started before one writes into another
-  const RowWalk at(q, p.cols, E);
-  const float inv_n = 1.f / static_cast<float>(p.cols);
-  const int rows = static_cast<int>(p.rows), step = at.step, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned long long key = RES && p.drop.on ? __ldg(p.drop.seed) : 0;
-  const int j0 = at.rank * q.chunk + at.t;
-  const uint32_t slots = sm100::smem_u32(ring) + warp * (q.per_thread * kOps * kUnit) + lane * 16;
-  constexpr uint32_t kStep = kMaxTeam * 16;
-
-  auto mask_of = [&](int k) { return column_mask<T, EDGE>(at, q, at.t + k * kMaxTeam, p.cols); };
-  const int mine = at.t < q.chunk ? (q.chunk - at.t + kMaxTeam - 1) / kMaxTeam : 0;      // granules of this thread, some perhaps empty
-  float count = 0.f;
-  for (int k = 0; k < mine; ++k) count += static_cast<float>(__popc(mask_of(k)));
-  count = warp_sum(count);
-  if (lane == 0) counts[warp] = count;
-
-  const int ends = last_rows<T, EDGE>(rows, p.cols);
-  auto fetch = [&](int row, int k) {
-    if (row >= rows || !mask_of(k)) return;
-    const size_t a = row_offset<T, EDGE>(row, p.ld_a, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
-    ring_copy(slots + (k * kOps) * kUnit, p.a, a, EDGE && row >= ends, p.rows * p.cols * sizeof(T));
-    if (RES) {
-      const size_t b = row_offset<T, EDGE>(row, p.ld_b, p.cols, j0) * sizeof(T) + static_cast<size_t>(k) * kStep;
-      ring_copy(slots + (k * kOps + 1) * kUnit, p.b, b, EDGE && row >= ends, p.rows * p.cols * sizeof(T));
-    }
-  };
-  // with a residual the sum is kept as fp32 in the granule's two slots
-  auto value = [&](int k, float2 (&v)[P]) {
-    if constexpr (RES) param_get<T>(slots + (k * kOps) * kUnit, v);
-    else ring_get<T>(slots + (k * kOps) * kUnit, v);
-  };
-
-  for (int k = 0; k < mine; ++k) fetch(at.first, k);
-  cp_async_commit();
-  __syncthreads();
-  int buf = 0;
-  for (int row = at.first; row < rows; row += step, buf ^= 1) {
-    const size_t out = row_offset<T, EDGE>(row, p.cols, p.cols, j0) * sizeof(T);
-    cp_async_wait(0);
-    float2 sum = both(0.f);
-#pragma unroll 4
-    for (int k = 0; k < mine; ++k) {
-      const uint32_t m = mask_of(k);
-      if (!m) continue;
-      float2 v[P];
-      ring_get<T>(slots + (k * kOps) * kUnit, v);
-      if (RES) {
-        float2 res[P];
-        ring_get<T>(slots + (k * kOps + 1) * kUnit, res);
-        if (p.drop.on) {
-          const size_t g[1] = {(out + static_cast<size_t>(k) * kStep) / 16};
-          Signs<T> gone[1];
-          granule_signs<T, 1>(p.drop, key, g, gone);
-          apply_signs<T>(v, gone[0], p.drop.scale);
-        }
-#pragma unroll
-        for (int i = 0; i < P; ++i) v[i] = add2(res[i], v[i]);
-        param_put<T>(slots + (k * kOps) * kUnit, v);
-      }
-      if (EDGE && m != kAll) zero_outside(v, m);
-#pragma unroll
-      for (int i = 0; i < P; ++i) sum = add2(sum, v[i]);
-    }
-    const float x = warp_sum(sum.x + sum.y), centre = count > 0.f ? x / count : 0.f;
-    float2 dev = both(0.f);
-#pragma unroll 4
-    for (int k = 0; k < mine; ++k) {
-      const uint32_t m = mask_of(k);
-      if (!m) continue;
-      float2 v[P];
-      value(k, v);
-      dev = deviations(v, centre, m, !EDGE || m == kAll, dev);
-    }
-    const float y = warp_sum(dev.x + dev.y);
-    if (lane == 0) red[buf][warp] = make_float2(x, y);
-    __syncthreads();
-    float mean, m2;
-    {
-      constexpr int kWarps = kMaxTeam / 32;
-      const float2 f = lane < kWarps ? red[buf][lane] : make_float2(0.f, 0.f);
-      const float c = lane < kWarps ? counts[lane] : 0.f;
-      const float total = warp_sum(f.x), n = warp_sum(c);
-      const float m = n > 0.f ? total / n : 0.f;
-      const float d = c > 0.f ? f.x / c - m : 0.f;
-      m2 = warp_sum(fmaf(c * d, d, f.y));
-      mean = m;
-      if (q.cluster > 1) {
-        if (threadIdx.x < q.cluster) {
-          put_remote(&peer[buf][at.rank][0], threadIdx.x, total);
-          put_remote(&peer[buf][at.rank][1], threadIdx.x, m2);
-          put_remote(&peer[buf][at.rank][2], threadIdx.x, n);
-        }
-        cluster_barrier();
-        const bool have = lane < q.cluster;
-        const float ps = have ? peer[buf][lane][0] : 0.f, pq = have ? peer[buf][lane][1] : 0.f, pn = have ? peer[buf][lane][2] : 0.f;
-        mean = warp_sum(ps) * inv_n;
-        const float pd = pn > 0.f ? ps / pn - mean : 0.f;
-        m2 = warp_sum(fmaf(pn * pd, pd, pq));
-      }
-    }
-    const float rstd = 1.f / sqrtf(m2 * inv_n + p.eps);
-    if (threadIdx.x == 0 && at.rank == 0) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-#pragma unroll 4
-    for (int k = 0; k < mine; ++k) {
-      const uint32_t m = mask_of(k);
-      if (!m) continue;
-      const long long col = static_cast<long long>(j0 + k * kMaxTeam) * E - at.m;
-      float2 v[P], w[P], b[P];
-      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, m, 1.f, w);
-      load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, m, 0.f, b);
-      value(k, v);
-      const size_t e = out + static_cast<size_t>(k) * kStep;
-      if (RES && p.out2) store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out2) + e), v, m);
-      normalise(v, mean, rstd, w, b);
-      store_granule<T, EDGE>(reinterpret_cast<T*>(static_cast<char*>(p.out) + e), v, m);
-      fetch(row + step, k);
-    }
-    cp_async_commit();
+// The statistics of a long row from those of its chunks: a warp a row.
+__global__ void __launch_bounds__(kBlock) ln_fwd_combine(const float* partial, int chunks, LnArgs p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const size_t row = static_cast<size_t>(blockIdx.x) * (kBlock / 32) + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const float* f = partial + row * chunks * 3;
+  float s = 0.f, q = 0.f;
+  for (int i = lane; i < chunks; i += 32) s += f[3 * i];
+  const float mean = warp_sum(s) / static_cast<float>(p.cols);
+  for (int i = lane; i < chunks; i += 32) {
+    const float n = f[3 * i + 2], d = n > 0.f ? f[3 * i] / n - mean : 0.f;
+    q += fmaf(n * d, d, f[3 * i + 1]);
   }
-  if (q.cluster > 1) cluster_barrier();      // no CTA leaves while a peer may still write into it
+  q = warp_sum(q);
+  if (lane == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = 1.f / sqrtf(q / static_cast<float>(p.cols) + p.eps);
+  }
 }
 
 template <typename T>
@@ -420,41 +337,42 @@ __global__ void __launch_bounds__(kBlock) ln_fwd_any(LnArgs p) {
 }
 
 
-template <typename Kernel>
-int launch_fwd(Kernel kernel, std::atomic<int>* cache, const LnArgs& p, RowPlan q, cudaStream_t st) {
+template <typename T, int K, bool RES, bool EDGE, int PASS>
+int launch_fwd(const LnArgs& p, RowPlan q, float* partial, cudaStream_t st) {
+  static std::atomic<int> cache[64];
+  auto kernel = ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE, PASS>;
   int regs = 0;
   if (int rc = prepare("layer_norm_fwd", kernel, cache, &regs)) return rc;
   size_grid(p.rows, resident(q.groups * q.team, regs, q.smem), &q);
-  if (!fit_clusters(kernel, &q)) return kDoesNotFit;
-  return launch_rows("layer_norm_fwd", kernel, q, st, p, q);
-}
-
-template <typename T, int K, bool RES, bool EDGE, bool CLUSTER>
-int rows_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
-  static std::atomic<int> cache[64];
-  return launch_fwd(ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE, CLUSTER>, cache, p, q, st);
-}
-
-template <typename T, bool RES, bool EDGE>
-int long_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
-  static std::atomic<int> cache[64];
-  return launch_fwd(ln_fwd_long<T, RES, EDGE>, cache, p, q, st);
+  if (PASS == kCluster && !fit_clusters(kernel, &q)) return kDoesNotFit;
+  return launch_rows("layer_norm_fwd", PASS, kernel, q, st, p, q, partial);
 }
 
 template <typename T, bool RES, bool EDGE>
 int pick_fwd(const LnArgs& p, const RowPlan& q, cudaStream_t st) {
-  if (q.cluster > 1)
-    return q.per_thread * kE<T> == 16 ? rows_fwd<T, 16 / kE<T>, RES, EDGE, true>(p, q, st) : rows_fwd<T, 32 / kE<T>, RES, EDGE, true>(p, q, st);
+  if (q.cluster > 1) return launch_fwd<T, 32 / kE<T>, RES, EDGE, kCluster>(p, q, nullptr, st);
   switch (q.per_thread) {
-    case 1: return rows_fwd<T, 1, RES, EDGE, false>(p, q, st);
-    case 2: return rows_fwd<T, 2, RES, EDGE, false>(p, q, st);
-    case 4: return rows_fwd<T, 4, RES, EDGE, false>(p, q, st);
-    default: return rows_fwd<T, 32 / kE<T>, RES, EDGE, false>(p, q, st);
+    case 1: return launch_fwd<T, 1, RES, EDGE, kWhole>(p, q, nullptr, st);
+    case 2: return launch_fwd<T, 2, RES, EDGE, kWhole>(p, q, nullptr, st);
+    case 4: return launch_fwd<T, 4, RES, EDGE, kWhole>(p, q, nullptr, st);
+    default: return launch_fwd<T, 32 / kE<T>, RES, EDGE, kWhole>(p, q, nullptr, st);
   }
 }
 
+template <typename T, bool RES, bool EDGE>
+int long_fwd(const LnArgs& p, const RowPlan& q, float* partial, cudaStream_t st) {
+  if (int rc = launch_fwd<T, 16 / kE<T>, RES, EDGE, kStats>(p, q, partial, st)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + kBlock / 32 - 1) / (kBlock / 32)));
+  cfg.blockDim = dim3(kBlock);
+  cfg.stream = st;
+  launch_dependent(&cfg, ln_fwd_combine, static_cast<const float*>(partial), q.cluster, p);
+  if (int rc = after_launch("layer_norm_fwd_combine")) return rc;
+  return launch_fwd<T, 16 / kE<T>, RES, EDGE, kApply>(p, q, nullptr, st);
+}
+
 template <typename T>
-int fwd(const LnArgs& p, bool granules, cudaStream_t st) {
+int fwd(const LnArgs& p, bool granules, float* ws, cudaStream_t st) {
   RowPlan q;
   const int ops = p.b ? 2 : 1;
   const bool edge = p.cols % kE<T> != 0;
@@ -463,9 +381,9 @@ int fwd(const LnArgs& p, bool granules, cudaStream_t st) {
     if (p.b) rc = edge ? pick_fwd<T, true, true>(p, q, st) : pick_fwd<T, true, false>(p, q, st);
     else rc = edge ? pick_fwd<T, false, true>(p, q, st) : pick_fwd<T, false, false>(p, q, st);
   }
-  if (rc == kDoesNotFit && granules && plan_fwd_long(p.rows, p.cols, sizeof(T), ops, &q)) {
-    if (p.b) rc = edge ? long_fwd<T, true, true>(p, q, st) : long_fwd<T, true, false>(p, q, st);
-    else rc = edge ? long_fwd<T, false, true>(p, q, st) : long_fwd<T, false, false>(p, q, st);
+  if (rc == kDoesNotFit && granules && plan_long(p.rows, p.cols, sizeof(T), ops, 2, &q)) {
+    if (p.b) rc = edge ? long_fwd<T, true, true>(p, q, ws, st) : long_fwd<T, true, false>(p, q, ws, st);
+    else rc = edge ? long_fwd<T, false, true>(p, q, ws, st) : long_fwd<T, false, false>(p, q, ws, st);
   }
   if (rc != kDoesNotFit) return rc;
   ln_fwd_any<T><<<grid_for(p.rows, 1, 8), kBlock, 0, st>>>(p);
@@ -479,9 +397,22 @@ using namespace mb;
 
 extern "C" {
 
+size_t mb_layer_norm_fwd_workspace_bytes(const mb_ln_desc* d) {
+  if (!d || d->cols == 0 || d->cols > 0x7fffffffULL || d->rows == 0 || !dtype_bytes(d->dtype)) return 0;
+  size_t floats = 0;
+  for (int ops = 1; ops <= 2; ++ops) {      // three values a chunk, for rows that one team or cluster does not hold
+    RowPlan q;
+    if (plan_fwd_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, &q) && q.cluster == 1) continue;
+    if (!plan_long(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, 2, &q)) continue;
+    const size_t n = d->rows * q.cluster * 3;
+    if (n > floats) floats = n;
+  }
+  return floats * sizeof(float);
+}
+
 int mb_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias, void* y,
                       void* sum, float* mean, float* rstd, const mb_ln_desc* d, const mb_dropout_desc* drop,
-                      void* stream) {
+                      void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "mb_layer_norm_fwd";
   if (int rc = check_desc(who, d)) return rc;
   LnArgs p{x, residual, nullptr, weight, bias, y, sum, mean, rstd, d->rows, d->cols, d->ld_a, d->ld_b, 0, d->param_dtype == MB_F32, aligned(weight, 16) && aligned(bias, 16), d->eps, {}};
@@ -492,11 +423,15 @@ int mb_layer_norm_fwd(const void* x, const void* residual, const void* weight, c
   if (!natural(d, x) || !natural(d, residual) || !natural(d, y) || !natural(d, sum) || !natural_param(d, weight) ||
       !natural_param(d, bias) || !aligned(mean, 4) || !aligned(rstd, 4))
     return fail(MB_ERR_INVALID_ARGUMENT, "%s: misaligned pointer", who);
+  const size_t need = mb_layer_norm_fwd_workspace_bytes(d);
+  if (need && (!workspace || !aligned(workspace, 4) || workspace_bytes < need))
+    return fail(MB_ERR_WORKSPACE, "%s: workspace too small or misaligned", who);
   cudaStream_t st = as_stream(stream);
+  float* ws = static_cast<float*>(workspace);
   const bool granules = on_granules(d, {{x, d->ld_a}, {residual, d->ld_b}, {y, d->cols}, {sum, d->cols}});
-  if (d->dtype == MB_F32) return fwd<float>(p, granules, st);
-  if (d->dtype == MB_BF16) return fwd<__nv_bfloat16>(p, granules, st);
-  return fwd<__half>(p, granules, st);
+  if (d->dtype == MB_F32) return fwd<float>(p, granules, ws, st);
+  if (d->dtype == MB_BF16) return fwd<__nv_bfloat16>(p, granules, ws, st);
+  return fwd<__half>(p, granules, ws, st);
 }
 
 }  // extern "C"

@@ -25,16 +25,20 @@ namespace mb {
 // Threads of a CTA: what the registers of an SM hold at 80 a thread, or 128 where a thread has 32 values.
 constexpr int kMaxThreads = 768, kMaxThreadsWide = 512;
 constexpr int kMaxTeam = 512;     // threads of a CTA that share a row (a CTA of a cluster: all of them)
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 4;    // 4 CTAs of 200 KB still fill 132 of 148 SMs, 8 only 120, 16 only 112
 constexpr int kUnit = 512;
 template <typename T> constexpr int kE = 16 / static_cast<int>(sizeof(T));    // elements of a granule
 template <typename T> constexpr int kPairs = kE<T> / 2;
+
+// How a kernel goes about a row: all of it by one team; by a cluster of CTAs; or, when it is long, a
+// chunk per CTA in two kernels, one for the row's statistics and one for the result.
+enum Pass { kWhole, kCluster, kStats, kApply };
 
 struct RowPlan {
   int team;        // threads of a CTA that share a row: a power of two up to 32, or a multiple of 32
   int groups;      // teams per CTA
   int per_thread;  // granules per thread (K of the kernel)
-  int cluster;     // CTAs that share a row (then groups == 1)
+  int cluster;     // CTAs that share a row (then groups == 1): a cluster, or the chunks of a long row
   int chunk;       // granules of a row per CTA
   int stages;      // rows in flight per team
   int period;
@@ -45,13 +49,14 @@ struct RowPlan {
 // Where a thread stands: its team, its rows (first, first + step, ...) and its granules.
 struct RowWalk {
   int group, t, rank, m, first, step;
-  __device__ __forceinline__ RowWalk(const RowPlan& q, size_t cols, int elems) {
+  // With `last` >= 0 the walk counts rows from that one backwards.
+  __device__ __forceinline__ RowWalk(const RowPlan& q, size_t cols, int elems, int last = -1) {
     group = threadIdx.x / q.team;
     t = threadIdx.x - group * q.team;
     const int cta = blockIdx.x / q.cluster;
     rank = blockIdx.x - cta * q.cluster;
     const int residue = cta % q.period;
-    m = static_cast<int>((static_cast<unsigned>(residue) * static_cast<unsigned>(cols)) & (elems - 1));
+    m = static_cast<int>((static_cast<unsigned>(last >= 0 ? last - residue : residue) * static_cast<unsigned>(cols)) & (elems - 1));
     step = static_cast<int>(gridDim.x / q.cluster / q.period) * q.groups * q.period;
     first = residue + q.period * (cta / q.period * q.groups + group);
   }
@@ -306,7 +311,7 @@ __device__ __forceinline__ void merge_lanes(float (&s)[N], float (&m2)[N], int l
       s[i] += t;
     }
 }
-// The N values of a row of `n` <= 16 rows of N floats in shared memory summed over the rows, by every lane.
+// The N values of a row of `n` rows of N floats (64 at most) in shared memory summed over the rows, by every lane.
 template <int N>
 __device__ __forceinline__ void gather(const float* f, int n, float (&s)[N]) {
   if (n <= 8) {        // few: every lane reads them all, without a chain of shuffles
@@ -319,7 +324,7 @@ __device__ __forceinline__ void gather(const float* f, int n, float (&s)[N]) {
   }
   const int lane = threadIdx.x & 31;
   float x = lane < N * n ? f[lane] : 0.f;
-  if (N * 16 > 32 && N * n > 32) x += lane + 32 < N * n ? f[lane + 32] : 0.f;
+  if (N * n > 32) x += lane + 32 < N * n ? f[lane + 32] : 0.f;
 #pragma unroll
   for (int o = N; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
 #pragma unroll

@@ -1080,8 +1080,10 @@ def _ln_desc(rows, cols, ld_a, ld_b, ld_c, code, param_code, eps):
 
 
 @functools.lru_cache(maxsize=4096)
-def _ln_workspace(device, rows, cols, code, param_code) -> int:
-    return lib().mb_layer_norm_workspace_bytes(C.byref(_ln_desc(rows, cols, cols, cols, cols, code, param_code, 0.0)))
+def _ln_workspace(device, rows, cols, code, param_code):
+    """Bytes of scratch (forward, backward)."""
+    d = C.byref(_ln_desc(rows, cols, cols, cols, cols, code, param_code, 0.0))
+    return lib().mb_layer_norm_fwd_workspace_bytes(d), lib().mb_layer_norm_bwd_workspace_bytes(d)
 
 
 def _as_rows(t: torch.Tensor, rows: int, cols: int):
@@ -1154,9 +1156,11 @@ def _layer_norm_fwd(x, residual, normalized_shape, weight, bias, eps, p, seed, o
     mean = torch.empty(rows, dtype=_F32, device=x.device)
     rstd = torch.empty(rows, dtype=_F32, device=x.device)
     d = _ln_desc(rows, cols, ld_a, ld_b, 0, code, _DTYPE_CODE[kind], eps)
+    nbytes = _ln_workspace(x.get_device(), rows, cols, code, _DTYPE_CODE[kind])[0]
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     check(lib().mb_layer_norm_fwd(xr.data_ptr(), _ptr(rr), _ptr(w), _ptr(b), y.data_ptr(), _ptr(z), mean.data_ptr(),
-                                  rstd.data_ptr(), C.byref(d), C.byref(drop) if drop is not None else None, _stream()),
-          "layer_norm_fwd")
+                                  rstd.data_ptr(), C.byref(d), C.byref(drop) if drop is not None else None, _ptr(ws), nbytes,
+                                  _stream()), "layer_norm_fwd")
     return y, z, mean, rstd
 
 
@@ -1183,14 +1187,12 @@ def _layer_norm_bwd(dy, kept, from_output, dz, normalized_shape, weight, bias, m
     dw = torch.empty(tail, dtype=kind, device=dy.device) if need_weight else None
     db = torch.empty(tail, dtype=kind, device=dy.device) if need_bias else None
     pcode = _DTYPE_CODE[kind]
-    ws, nbytes = None, 0
-    if need_weight or need_bias:
-        nbytes = _ln_workspace(dy.get_device(), rows, cols, code, pcode)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+    nbytes = _ln_workspace(dy.get_device(), rows, cols, code, pcode)[1]
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
     d = _ln_desc(rows, cols, cols, cols, cols, code, pcode, 0.0)
     check(lib().mb_layer_norm_bwd(gr.data_ptr(), kr.data_ptr(), from_output, _ptr(zr), _ptr(w), _ptr(b), _ptr(mean),
                                   rstd.data_ptr(), dv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), C.byref(d),
-                                  C.byref(drop) if drop is not None else None, _ptr(ws), nbytes, _stream()), "layer_norm_bwd")
+                                  C.byref(drop) if drop is not None else None, ws.data_ptr(), nbytes, _stream()), "layer_norm_bwd")
     return dv, dx, dw, db
 
 

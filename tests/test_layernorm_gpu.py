@@ -274,7 +274,7 @@ def test_backward_over_its_inputs(cuda):
         want = F.dropout_add_layer_norm_bwd_from_sum(dy, x, (cols,), w, mean, rstd, 0.2, seed, 3)
         d = _lib.LnDesc(rows, cols, cols, cols, 0, _lib.MB_BF16, _lib.MB_F32, 0.0)
         q = _lib.DropoutDesc(0.2, seed.data_ptr(), 3)
-        ws = torch.empty(_lib.lib().mb_layer_norm_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=cuda)
+        ws = torch.empty(_lib.lib().mb_layer_norm_bwd_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=cuda)
         dw, db = torch.empty(cols, device=cuda), torch.empty(cols, device=cuda)
         a, k = dy.clone(), x.clone()
         rc = _lib.lib().mb_layer_norm_bwd(a.data_ptr(), k.data_ptr(), 0, None, w.data_ptr(), None, mean.data_ptr(),

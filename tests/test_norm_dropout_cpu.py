@@ -145,9 +145,9 @@ def test_refused_before_any_launch(built_lib):
     api = _lib.lib()
     one = C.c_void_p(64)          # non-null and aligned: never dereferenced
 
-    def fwd(d, drop=None, x=one, residual=None, y=one):
+    def fwd(d, drop=None, x=one, residual=None, y=one, ws=None, nbytes=0):
         return api.mb_layer_norm_fwd(x, residual, None, None, y, None, one, one, C.byref(d) if d else None,
-                                     C.byref(drop) if drop else None, None)
+                                     C.byref(drop) if drop else None, ws, nbytes, None)
 
     def bwd(d, drop=None, ws=one, nbytes=0, dx=None, mean=one, out=0):
         return api.mb_layer_norm_bwd(one, one, out, None, None, None, mean, one, one, dx, one, one, C.byref(d),
@@ -174,8 +174,14 @@ def test_refused_before_any_launch(built_lib):
             (lambda: api.mb_dropout(one, one, 8, 0, C.byref(_lib.DropoutDesc(float("nan"), 64, 0)), None), 1, "probability")]:
         rc = call()
         assert rc == code and word in _lib.last_error(), (rc, code, word, _lib.last_error())
-    assert api.mb_layer_norm_workspace_bytes(C.byref(ok())) >= 2 * 16 * 4
-    assert api.mb_layer_norm_workspace_bytes(C.byref(ok(rows=0))) == 0
+    assert api.mb_layer_norm_bwd_workspace_bytes(C.byref(ok())) >= 2 * 16 * 4
+    assert api.mb_layer_norm_bwd_workspace_bytes(C.byref(ok(rows=0))) == 0 and api.mb_layer_norm_bwd_workspace_bytes(None) == 0
+    assert api.mb_layer_norm_fwd_workspace_bytes(C.byref(ok())) == 0
+    long = ok(cols=1 << 20, a=1 << 20, b=1 << 20)       # rows walked twice need room for their sums
+    need = api.mb_layer_norm_fwd_workspace_bytes(C.byref(long))
+    assert need > 0
+    for ws, nbytes in ((None, need), (one, need - 4), (C.c_void_p(66), need)):
+        assert fwd(long, ws=ws, nbytes=nbytes) == 3 and "workspace" in _lib.last_error()
 
 
 def test_cpu_tensors_are_refused(built_lib):
