@@ -589,6 +589,10 @@ int mb_layer_norm_bwd(const void* dy, const void* kept, int kept_is_output, cons
     return MB_OK;
   }
   if (!dy || !kept || !rstd || !dv || (!kept_is_output && !mean)) return fail(MB_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (dv == dx) return fail(MB_ERR_INVALID_ARGUMENT, "%s: dv and dx must not be the same buffer", who);
+  for (const void* o : {static_cast<const void*>(dv), static_cast<const void*>(dx)})
+    if (o && ((o == dy && d->ld_a != d->cols) || (o == kept && d->ld_b != d->cols) || (o == dsum && d->ld_c != d->cols)))
+      return fail(MB_ERR_INVALID_ARGUMENT, "%s: only dense rows can be overwritten", who);
   if (drop && !dx) return fail(MB_ERR_INVALID_ARGUMENT, "%s: dropout needs dx", who);
   if (!natural(d, dy) || !natural(d, kept) || !natural(d, dsum) || !natural(d, dv) || !natural(d, dx) || !aligned(mean, 4) || !aligned(rstd, 4))
     return fail(MB_ERR_INVALID_ARGUMENT, "%s: misaligned pointer", who);

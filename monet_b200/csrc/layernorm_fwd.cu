@@ -419,6 +419,9 @@ int mb_layer_norm_fwd(const void* x, const void* residual, const void* weight, c
   if (int rc = make_drop(who, drop, &p.drop)) return rc;
   if (d->rows == 0) return MB_OK;
   if (!x || !y || !mean || !rstd) return fail(MB_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (y == sum) return fail(MB_ERR_INVALID_ARGUMENT, "%s: y and sum must not be the same buffer", who);
+  if (((y == x || sum == x) && d->ld_a != d->cols) || (residual && (y == residual || sum == residual) && d->ld_b != d->cols))
+    return fail(MB_ERR_INVALID_ARGUMENT, "%s: only dense rows can be overwritten", who);
   if (drop && !residual) return fail(MB_ERR_INVALID_ARGUMENT, "%s: dropout needs a residual", who);
   if (!natural(d, x) || !natural(d, residual) || !natural(d, y) || !natural(d, sum) || !natural_param(d, weight) ||
       !natural_param(d, bias) || !aligned(mean, 4) || !aligned(rstd, 4))

@@ -16,7 +16,8 @@ EPS = 1e-5
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 SHAPES = [(1, 1), (3, 1), (5, 2), (4, 7), (1, 8), (2, 16), (37, 31), (64, 64), (9, 100), (33, 128), (7, 257), (130, 768),
           (50, 1000), (11, 1023), (3, 2047), (8, 2048), (5, 4096), (3, 4099), (2, 8192), (2, 12289), (3, 16384), (1, 1 << 15),
-          (2, 40000), (3, 65537), (1, 200704), (2, 300000), (2000, 72), (1201, 33), (700, 1024), (500, 2501)]
+          (2, 40000), (3, 65537), (1, 200704), (2, 300000), (2000, 72), (1201, 33), (700, 1024), (500, 2501),
+          (301, 20000), (299, 17001), (150, 66001), (40, 131080), (900, 8192), (640, 9999)]
 MIXES = [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f16", "f16")]
 
 
@@ -127,7 +128,7 @@ def test_forward_and_backward(cuda, rows, cols, mix):
 
 @pytest.mark.parametrize("mix", MIXES, ids="-".join)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (5, 7), (13, 64), (9, 100), (130, 768), (50, 1000), (11, 1023), (6, 4096), (3, 8200),
-                                       (2, 20001), (1201, 33), (3, 70000)])
+                                       (2, 20001), (1201, 33), (3, 70000), (150, 33001), (33, 131072)])
 @pytest.mark.parametrize("p", [0.0, 0.1, 0.5])
 def test_dropout_add_layer_norm(cuda, rows, cols, mix, p):
     """Forward with and without the sum, backward from the sum (with a gradient of its own) and from

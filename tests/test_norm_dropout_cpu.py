@@ -165,6 +165,8 @@ def test_refused_before_any_launch(built_lib):
             (lambda: fwd(ok(), _lib.DropoutDesc(1.5, 64, 0), residual=one), 1, "probability"),
             (lambda: fwd(ok(), _lib.DropoutDesc(0.5, None, 0), residual=one), 1, "seed"),
             (lambda: fwd(ok(), _lib.DropoutDesc(0.5, 68, 0), residual=one), 1, "seed"),
+            (lambda: fwd(ok(a=32), y=one, x=one), 1, "dense"), (lambda: fwd(ok(b=0), x=C.c_void_p(128), residual=one), 1, "dense"),
+            (lambda: bwd(ok(), dx=one, nbytes=1 << 20), 1, "same buffer"), (lambda: bwd(ok(a=32), nbytes=1 << 20), 1, "dense"),
             (lambda: bwd(ok()), 3, "workspace"), (lambda: bwd(ok(), ws=None, nbytes=1 << 20), 3, "workspace"),
             (lambda: bwd(ok(), mean=None, nbytes=1 << 20), 1, "null"),
             (lambda: bwd(ok(), _lib.DropoutDesc(0.5, 64, 0), nbytes=1 << 20), 1, "dx"),
