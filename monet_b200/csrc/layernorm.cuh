@@ -55,6 +55,10 @@ inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b -
 // Rows between two barriers of the backward kernel with k granules a thread.
 constexpr int bwd_rows_between_barriers(int k) { return k == 1 ? 2 : 1; }
 constexpr int fwd_rows_between_barriers(int k, int elems) { return k == 1 ? 2 : 1; }
+// Threads of a forward CTA: 32 values a thread fit 80 registers in the plain form alone.
+constexpr int fwd_threads(int k, int elems, bool residual, bool edge) {
+  return k * elems >= 32 && residual ? kMaxThreadsWide : kMaxThreads;
+}
 
 // The period of the rows' alignment, and the granules that a row can touch.
 inline size_t row_granules(size_t cols, int elems, int* period) {
@@ -164,7 +168,7 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
     if (q->team > kMaxTeam) continue;
     const int r = fwd_rows_between_barriers(q->per_thread, elems);
     const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
-    for (int teams = cta_threads(*q, elems) / q->team; teams >= 1; --teams) {
+    for (int teams = fwd_threads(q->per_thread, elems, ops == 2, cols % elems != 0) / q->team; teams >= 1; --teams) {
       plan_groups(rows, teams, q);
       if (plan_ring(rows, r, ops, 2, params, q)) return true;
     }

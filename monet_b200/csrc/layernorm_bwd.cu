@@ -96,22 +96,23 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
       if (at.first + (s + r) * step < rows) fetch(slots + (s + r) * stride, at.first + (s + r) * step, out + (s + r) * out_step);
     cp_async_commit();
   }
-  if (kInRegs || at.group == 0) {
+  // every thread brings some granules' parameters, whichever teams they are for
+  for (int i = kInRegs ? at.t : static_cast<int>(threadIdx.x); i < (kInRegs ? at.t + 1 : K * q.team); i += blockDim.x) {
+    const uint32_t m = column_mask<T, EDGE>(at, q, i, p.cols);
+    const long long col = static_cast<long long>(at.rank * q.chunk + i) * E - at.m;
+    const int k = i / q.team, t = i - k * q.team;
+    const uint32_t to = sm100::smem_u32(ring) + q.stages * stride + (t >> 5) * (K * kKinds * kParam) + (t & 31) * 16 + k * kKinds * kParam;
+    float2 v[P];
+    load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, m, 1.f, v);
+    if constexpr (kInRegs) copy_pairs(v, wr); else param_put<T>(to, v);
+    if (FROM_Y) {
+      load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, m, 0.f, v);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
-      float2 v[P];
-      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, v);
-      if constexpr (kInRegs) copy_pairs(v, wr); else param_put<T>(params + (k * kKinds) * kParam, v);
-      if (FROM_Y) {
-        load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, v);
-#pragma unroll
-        for (int i = 0; i < P; ++i) v[i] = make_float2(-v[i].x, -v[i].y);
-        if constexpr (kInRegs) copy_pairs(v, nbr); else param_put<T>(params + (k * kKinds + 1) * kParam, v);
-      }
+      for (int j = 0; j < P; ++j) v[j] = make_float2(-v[j].x, -v[j].y);
+      if constexpr (kInRegs) copy_pairs(v, nbr); else param_put<T>(to + kParam, v);
     }
   }
-  if (!kInRegs && q.groups > 1) __syncthreads();   // the parameters that group 0 put down
+  if (!kInRegs) __syncthreads();
 
   int row = at.first;
   const int spare = at.spare(q);

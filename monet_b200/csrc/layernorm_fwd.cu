@@ -26,7 +26,7 @@ __device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, u
 }
 
 template <typename T, int K, int R, bool RES, bool EDGE, int PASS>
-__global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThreads) ln_fwd_rows(LnArgs p, RowPlan q, float* partial) {
+__global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES, EDGE)) ln_fwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
   __shared__ float counts[kMaxThreads / 32];
@@ -96,19 +96,20 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   }
 
   float2 wr[P], br[P];
-  if (PASS != kStats && (kInRegs || at.group == 0)) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long col = static_cast<long long>(j0 + k * q.team) * E - at.m;
-      load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, mask[k], 1.f, wr);
-      load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, mask[k], 0.f, br);
-      if (!kInRegs) {
-        param_put<T>(params + (2 * k) * kParam, wr);
-        param_put<T>(params + (2 * k + 1) * kParam, br);
-      }
+  // every thread brings some granules' parameters, whichever teams they are for
+  for (int i = kInRegs ? at.t : static_cast<int>(threadIdx.x); PASS != kStats && i < (kInRegs ? at.t + 1 : K * q.team); i += blockDim.x) {
+    const uint32_t m = column_mask<T, EDGE>(at, q, i, p.cols);
+    const long long col = static_cast<long long>(at.rank * q.chunk + i) * E - at.m;
+    const int k = i / q.team, t = i - k * q.team;
+    const uint32_t to = sm100::smem_u32(ring) + q.stages * stride + (t >> 5) * (K * 2 * kParam) + (t & 31) * 16 + 2 * k * kParam;
+    load_params<T>(p.w, p.w_f32, p.w_vec && !EDGE, col, m, 1.f, wr);
+    load_params<T>(p.bias, p.w_f32, p.w_vec && !EDGE, col, m, 0.f, br);
+    if (!kInRegs) {
+      param_put<T>(to, wr);
+      param_put<T>(to + kParam, br);
     }
   }
-  if (!kInRegs) __syncthreads();       // the parameters that group 0 put down, and the counts
+  if (!kInRegs) __syncthreads();       // the parameters and the counts
   // Combining the warps' statistics, a lane looks after the warp of its number.  Warps with equal counts,
   // a power of two of them, merge like lanes.
   const bool alike = !EDGE && q.chunk == K * q.team && (warps & (warps - 1)) == 0;

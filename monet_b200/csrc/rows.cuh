@@ -333,10 +333,10 @@ __device__ __forceinline__ void gather(const float* f, int n, float (&s)[N]) {
 // Over aligned groups of `lanes` (a power of two up to 32).
 template <int N>
 __device__ __forceinline__ void lanes_sums(float (&s)[N], int lanes) {
-  if (lanes == 32 && N > 1) {
+  if (lanes == 32) {
     const float x = warp_sums(s);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = __shfl_sync(0xffffffffu, x, i * (32 / N));
+    for (int i = 0; i < N; ++i) s[i] = N == 1 ? x : __shfl_sync(0xffffffffu, x, i * (32 / N));
     return;
   }
   for (int o = lanes >> 1; o > 0; o >>= 1)
