@@ -89,6 +89,12 @@ inline int one_warp_values(int chunk, int elems) {
   while (v < 32 && chunk * elems > 32 * v) v *= 2;
   return chunk * elems <= 32 * v ? v : 0;
 }
+// 32 values a thread, or 16 where whole warps of 32 would leave a quarter more of their slots empty (1023
+// 16-bit values that start inside a granule touch 129: one more than a warp's).
+inline int wide_values(int chunk, int elems) {
+  const int wide = ceil_div(chunk, 1024 / elems) * (1024 / elems), narrow = ceil_div(chunk, 512 / elems) * (512 / elems);
+  return wide * 4 > narrow * 5 && narrow / (16 / elems) <= kMaxTeam ? 16 : 32;
+}
 inline int cta_threads(const RowPlan& q, int elems) { return q.per_thread * elems >= 32 ? kMaxThreadsWide : kMaxThreads; }
 
 // Teams per CTA: at most `most`, or as few as give no team more rows than that would.
@@ -134,7 +140,7 @@ inline bool plan_bwd_rows(size_t rows, size_t cols, int elem, int ops, bool from
     // 70 us with four teams of 128, 74 with three of 256).
     int teams = deep >= 6 ? static_cast<int>(deep / 3) : deep >= 5 ? 2 : 1, values = q->cluster > 1 ? 32 : one_warp_values(chunk, elems);
     if (!values) {
-      values = 32;
+      values = wide_values(chunk, elems);
       while (values > 8 && values > 2 * elems && static_cast<long long>(chunk) * elems / values * teams < 512 &&
              static_cast<long long>(chunk) * elems * 2 / values <= kMaxTeam)
         values /= 2;
@@ -163,7 +169,7 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
   for (q->cluster = 1; q->cluster <= kMaxCluster; q->cluster *= 2) {
     const int chunk = ceil_div(static_cast<long long>(most), q->cluster);
     int values = q->cluster > 1 ? 32 : one_warp_values(chunk, elems);
-    if (!values) values = 32;      // (16384 x 8192 bf16: 107 us against 154 with 16)
+    if (!values) values = wide_values(chunk, elems);      // (16384 x 8192 bf16: 107 us with 32 against 154 with 16)
     plan_team(chunk, elems, values, q);
     if (q->team > kMaxTeam) continue;
     const int r = fwd_rows_between_barriers(q->per_thread, elems);
