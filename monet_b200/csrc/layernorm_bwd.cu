@@ -12,7 +12,7 @@ namespace {
 // (in registers where a thread has one granule).  With 80 registers a thread, 24 warps share an SM,
 // and one team computes while another waits for its barrier.
 //
-// Long rows (PASS): kStats writes the two sums of each chunk, sums_of_rows[row][chunk][2]; kApply finds
+// Long rows (PASS): kStats writes the two sums of each chunk's warps, sums_of_rows[row][chunk][warp][2]; kApply finds
 // the rows' sums there, [row][2], and forms dv and the column sums in one reading.
 //
 // With t = v - mean or y - b:  sum g xhat = rstd sum (dy t) w  or  sum dy t  (the weight cancels), and
@@ -160,7 +160,11 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
       s[2 * r] = t1[r].x + t1[r].y;
       s[2 * r + 1] = t2[r].x + t2[r].y;
     }
-    if (q.team <= 32) {
+    if constexpr (PASS == kStats) {      // every warp leaves its own: no barrier
+      const float x = warp_sums(s);
+      if ((threadIdx.x & (16 / R - 1)) == 0 && row < rows)
+        sums_of_rows[((static_cast<size_t>(row) * q.cluster + at.rank) * (q.team >> 5) + (threadIdx.x >> 5)) * 2 + (threadIdx.x & 31) / (16 / R)] = x;
+    } else if (q.team <= 32) {
       lanes_sums(s, q.team);
     } else {
       const float x = warp_sums(s);
@@ -175,16 +179,6 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
         gather(peer[buf][0], q.cluster, s);
       }
     }
-      if constexpr (PASS == kStats) {
-        if (threadIdx.x == 0)
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-            if (row + r * step < rows) {
-              float* to = sums_of_rows + (static_cast<size_t>(row + r * step) * q.cluster + at.rank) * 2;
-              to[0] = s[2 * r];
-              to[1] = s[2 * r + 1];
-            }
-      }
     } else {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -331,20 +325,20 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
   }
 }
 
-// The sums of a long row from those of its chunks: a warp a row, into [row][2].
-__global__ void __launch_bounds__(kBlock) ln_bwd_combine(const float* chunk_sums, int chunks, size_t rows, float* row_sums) {
+// The sums of a long row from those of its `parts`: a CTA a row, into [row][2].
+__global__ void __launch_bounds__(kBlock) ln_bwd_combine(const float* part_sums, int parts, float* row_sums) {
+  __shared__ float red[kBlock / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const size_t row = static_cast<size_t>(blockIdx.x) * (kBlock / 32) + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  const size_t row = blockIdx.x;
+  const float2* f = reinterpret_cast<const float2*>(part_sums) + row * parts;
   float a = 0.f, b = 0.f;
-  for (int i = lane; i < chunks; i += 32) {
-    a += chunk_sums[(row * chunks + i) * 2];
-    b += chunk_sums[(row * chunks + i) * 2 + 1];
+  for (int i = threadIdx.x; i < parts; i += kBlock) {
+    a += f[i].x;
+    b += f[i].y;
   }
-  a = warp_sum(a);
-  b = warp_sum(b);
-  if (lane == 0) {
+  a = block_sum(a, red);
+  b = block_sum(b, red);
+  if (threadIdx.x == 0) {
     row_sums[2 * row] = a;
     row_sums[2 * row + 1] = b;
   }
@@ -509,13 +503,13 @@ template <typename T, bool FROM_Y, bool DSUM, bool DROP, bool EDGE>
 int long_bwd(const LnArgs& p, const RowPlan& q, const Grads& g, cudaStream_t st) {
   constexpr int K = 16 / kE<T>;
   float* row_sums = g.ws + static_cast<size_t>(q.grid / q.cluster) * 2 * p.cols;
-  float* chunk_sums = row_sums + 2 * p.rows;
+  float* chunk_sums = row_sums + 2 * p.rows;      // (8-byte aligned, as cols * 2 and rows * 2 are even)
   if (int rc = launch_bwd<T, K, FROM_Y, false, false, EDGE, kStats>(p, q, g, st, chunk_sums)) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + kBlock / 32 - 1) / (kBlock / 32)));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows));
   cfg.blockDim = dim3(kBlock);
   cfg.stream = st;
-  launch_dependent(&cfg, ln_bwd_combine, static_cast<const float*>(chunk_sums), q.cluster, p.rows, row_sums);
+  launch_dependent(&cfg, ln_bwd_combine, static_cast<const float*>(chunk_sums), q.cluster * (q.team / 32), row_sums);
   if (int rc = after_launch("layer_norm_bwd_combine")) return rc;
   return launch_bwd<T, K, FROM_Y, DSUM, DROP, EDGE, kApply>(p, q, g, st, row_sums);
 }
@@ -565,7 +559,7 @@ size_t mb_layer_norm_bwd_workspace_bytes(const mb_ln_desc* d) {
     if (fits) n = static_cast<size_t>(q.grid / q.cluster) * 2 * d->cols;
     if (n > floats) floats = n;
     if ((!fits || q.cluster > 1) && plan_bwd_long(d, 2 + form / 2, form % 2, &q))
-      n = static_cast<size_t>(q.grid / q.cluster) * 2 * d->cols + 2 * d->rows * (1 + static_cast<size_t>(q.cluster));
+      n = static_cast<size_t>(q.grid / q.cluster) * 2 * d->cols + 2 * d->rows * (1 + static_cast<size_t>(q.cluster) * (q.team / 32));
     if (n > floats) floats = n;
   }
   return floats * sizeof(float);

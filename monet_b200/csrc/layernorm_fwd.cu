@@ -192,7 +192,14 @@ __global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES, EDGE)) ln_fwd_rows(
       spread(mean, false);
       lanes_sums(m2, kInRegs ? q.team : 32);
     }
-    if (q.team > 32) {
+    if constexpr (PASS == kStats) {      // every warp leaves its own: no barrier
+      if (lane == 0 && row < rows) {
+        float* to = partial + ((static_cast<size_t>(row) * q.cluster + at.rank) * warps + (threadIdx.x >> 5)) * 3;
+        to[0] = s[0];
+        to[1] = m2[0];
+        to[2] = count;
+      }
+    } else if (q.team > 32) {
       if (lane == 0)
 #pragma unroll
         for (int r = 0; r < R; ++r) red[buf][threadIdx.x >> 5][r] = make_float2(s[r], m2[r]);
@@ -224,12 +231,6 @@ __global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES, EDGE)) ln_fwd_rows(
           total = warp_sum(ps);
           const float d = pn > 0.f ? ps / pn - total * inv_n : 0.f;
           sq = warp_sum(fmaf(pn * d, d, pq));
-        }
-        if (PASS == kStats && threadIdx.x == 0 && row + r * step < rows) {
-          float* to = partial + (static_cast<size_t>(row + r * step) * q.cluster + at.rank) * 3;
-          to[0] = total;
-          to[1] = sq;
-          to[2] = n;
         }
         s[r] = total;
         m2[r] = sq;
@@ -279,24 +280,24 @@ __global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES, EDGE)) ln_fwd_rows(
   if (PASS == kCluster) cluster_barrier();      // no CTA leaves while a peer may still write into it
 }
 
-// The statistics of a long row from those of its chunks: a warp a row.
-__global__ void __launch_bounds__(kBlock) ln_fwd_combine(const float* partial, int chunks, LnArgs p) {
+// The statistics of a long row from those of its `parts`: a CTA a row.
+__global__ void __launch_bounds__(kBlock) ln_fwd_combine(const float* partial, int parts, LnArgs p) {
+  __shared__ float red[kBlock / 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const size_t row = static_cast<size_t>(blockIdx.x) * (kBlock / 32) + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  const float* f = partial + row * chunks * 3;
+  const size_t row = blockIdx.x;
+  const float* f = partial + row * parts * 3;
+  const float inv_n = 1.f / static_cast<float>(p.cols);
   float s = 0.f, q = 0.f;
-  for (int i = lane; i < chunks; i += 32) s += f[3 * i];
-  const float mean = warp_sum(s) / static_cast<float>(p.cols);
-  for (int i = lane; i < chunks; i += 32) {
+  for (int i = threadIdx.x; i < parts; i += kBlock) s += f[3 * i];
+  const float mean = block_sum(s, red) * inv_n;
+  for (int i = threadIdx.x; i < parts; i += kBlock) {
     const float n = f[3 * i + 2], d = n > 0.f ? f[3 * i] / n - mean : 0.f;
     q += fmaf(n * d, d, f[3 * i + 1]);
   }
-  q = warp_sum(q);
-  if (lane == 0) {
+  q = block_sum(q, red);
+  if (threadIdx.x == 0) {
     p.mean[row] = mean;
-    p.rstd[row] = 1.f / sqrtf(q / static_cast<float>(p.cols) + p.eps);
+    p.rstd[row] = 1.f / sqrtf(q * inv_n + p.eps);
   }
 }
 
@@ -364,10 +365,10 @@ template <typename T, bool RES, bool EDGE>
 int long_fwd(const LnArgs& p, const RowPlan& q, float* partial, cudaStream_t st) {
   if (int rc = launch_fwd<T, 16 / kE<T>, RES, EDGE, kStats>(p, q, partial, st)) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.rows + kBlock / 32 - 1) / (kBlock / 32)));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows));
   cfg.blockDim = dim3(kBlock);
   cfg.stream = st;
-  launch_dependent(&cfg, ln_fwd_combine, static_cast<const float*>(partial), q.cluster, p);
+  launch_dependent(&cfg, ln_fwd_combine, static_cast<const float*>(partial), q.cluster * (q.team / 32), p);
   if (int rc = after_launch("layer_norm_fwd_combine")) return rc;
   return launch_fwd<T, 16 / kE<T>, RES, EDGE, kApply>(p, q, nullptr, st);
 }
@@ -401,11 +402,11 @@ extern "C" {
 size_t mb_layer_norm_fwd_workspace_bytes(const mb_ln_desc* d) {
   if (!d || d->cols == 0 || d->cols > 0x7fffffffULL || d->rows == 0 || !dtype_bytes(d->dtype)) return 0;
   size_t floats = 0;
-  for (int ops = 1; ops <= 2; ++ops) {      // three values a chunk, for rows that one team or cluster does not hold
+  for (int ops = 1; ops <= 2; ++ops) {      // three values a warp, for rows that one team or cluster does not hold
     RowPlan q;
     if (plan_fwd_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, &q) && q.cluster == 1) continue;
     if (!plan_long(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, 2, &q)) continue;
-    const size_t n = d->rows * q.cluster * 3;
+    const size_t n = d->rows * q.cluster * (q.team / 32) * 3;
     if (n > floats) floats = n;
   }
   return floats * sizeof(float);
