@@ -1,6 +1,7 @@
 // Dropout from the counter-based generator (philox.cuh).  The backward is the same map applied to
 // the gradient.  Bound by HBM: it reads and writes each element once; the generator's ten rounds per
-// eight elements stay below that.
+// eight elements stay below that.  67 million bf16 values 48 us (0.86 of a copy at 6569 GB/s), as many
+// fp32 values 84 us (0.97).
 #include <type_traits>
 #include "philox.cuh"
 #include "types.cuh"

@@ -8,6 +8,13 @@
 //
 // Everything is computed in fp32; outputs are rounded once.  Sums over rows are made in a fixed
 // order: per-CTA partials in the workspace, then one reduction.
+//
+// Bound by HBM for large tensors: forward reads and writes each element once, backward reads two or
+// three tensors and writes one or two.  Measured against a copy at 6569 GB/s: forward bf16 16384 x 8192
+// 88 us (0.93), 16384 x 4096 50 us (0.82); backward bf16 16384 x 4096 70 us (0.87), fp32 144256 x 128 from
+// the output 41 us (0.83); with dropout, add and sum bf16 8192 x 2048 forward 32 us (0.64), backward 45 us
+// (0.57), where the generator's instructions and the latency of a row's reductions are what is left.
+// Small calls (a few microseconds) are bound by their launches.
 #pragma once
 #include <atomic>
 #include <initializer_list>
@@ -54,9 +61,10 @@ constexpr size_t kSmemLimit = 225 * 1024;
 inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 // Rows between two barriers of the backward kernel with k granules a thread.
 constexpr int bwd_rows_between_barriers(int k) { return k == 1 ? 2 : 1; }
-constexpr int fwd_rows_between_barriers(int k, int elems) { return k == 1 ? 2 : 1; }
-// Threads of a forward CTA: 32 values a thread fit 80 registers in the plain form alone.
-constexpr int fwd_threads(int k, int elems, bool residual, bool edge) {
+constexpr int fwd_rows_between_barriers(int k) { return k == 1 ? 2 : 1; }
+// Threads of a forward CTA: 32 values a thread fit 80 registers in the plain form alone (768 threads
+// instead of 512: bf16 16384 x 8192 107 -> 89 us).
+constexpr int fwd_threads(int k, int elems, bool residual) {
   return k * elems >= 32 && residual ? kMaxThreadsWide : kMaxThreads;
 }
 
@@ -172,9 +180,9 @@ inline bool plan_fwd_rows(size_t rows, size_t cols, int elem, int ops, RowPlan* 
     if (!values) values = wide_values(chunk, elems);      // (16384 x 8192 bf16: 107 us with 32 against 154 with 16)
     plan_team(chunk, elems, values, q);
     if (q->team > kMaxTeam) continue;
-    const int r = fwd_rows_between_barriers(q->per_thread, elems);
+    const int r = fwd_rows_between_barriers(q->per_thread);
     const size_t params = q->per_thread == 1 ? 0 : static_cast<size_t>(q->team) * q->per_thread * elems * 8;
-    for (int teams = fwd_threads(q->per_thread, elems, ops == 2, cols % elems != 0) / q->team; teams >= 1; --teams) {
+    for (int teams = fwd_threads(q->per_thread, elems, ops == 2) / q->team; teams >= 1; --teams) {
       plan_groups(rows, teams, q);
       if (plan_ring(rows, r, ops, 2, params, q)) return true;
     }

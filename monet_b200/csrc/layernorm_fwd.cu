@@ -8,7 +8,10 @@ namespace {
 // Statistics: every thread centres on its own mean, and (sum, squared deviations) are merged pairwise
 // over the lanes, then over the warps and the CTAs of a cluster: no difference of large sums is ever
 // formed, and one pass over the lanes does.  (Where a warp's lanes hold different numbers of values it
-// centres on the warp's mean instead.)
+// centres on the warp's mean instead.)  The chain of shuffles is what a row waits for: bf16 16384 x 4096
+// took 63 us with one pass for the mean and one for the deviations, 57 with the merge.
+// Long rows (PASS): 184 x 200704 fp32 takes 80 us in two passes; held in the shared memory of clusters of
+// eight or sixteen CTAs it took 100, since those leave a fifth of the SMs without work.
 template <int P>
 __device__ __forceinline__ void normalise(float2 (&y)[P], float mean, float rstd, const float2 (&w)[P], const float2 (&b)[P]) {
 #pragma unroll
@@ -26,7 +29,7 @@ __device__ __forceinline__ float2 deviations(const float2 (&v)[P], float mean, u
 }
 
 template <typename T, int K, int R, bool RES, bool EDGE, int PASS>
-__global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES, EDGE)) ln_fwd_rows(LnArgs p, RowPlan q, float* partial) {
+__global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES)) ln_fwd_rows(LnArgs p, RowPlan q, float* partial) {
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ float2 red[2][kMaxThreads / 32][R];      // double-buffered by row: one barrier a row
   __shared__ float counts[kMaxThreads / 32];
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(kBlock) ln_fwd_any(LnArgs p) {
 template <typename T, int K, bool RES, bool EDGE, int PASS>
 int launch_fwd(const LnArgs& p, RowPlan q, float* partial, cudaStream_t st) {
   static std::atomic<int> cache[64];
-  auto kernel = ln_fwd_rows<T, K, fwd_rows_between_barriers(K, kE<T>), RES, EDGE, PASS>;
+  auto kernel = ln_fwd_rows<T, K, fwd_rows_between_barriers(K), RES, EDGE, PASS>;
   int regs = 0;
   if (int rc = prepare("layer_norm_fwd", kernel, cache, &regs)) return rc;
   size_grid(p.rows, resident(q.groups * q.team, regs, q.smem), &q);

@@ -12,8 +12,8 @@
 // ahead), so the ring needs no barrier: waiting for one's own copies is enough.  A warp's part of a
 // stage is a block of units of 512 bytes, 16 a lane, one unit for each (granule, operand): a thread
 // reaches all of its slots by constant offsets from one address, and neighbouring lanes always touch
-// neighbouring 16 bytes (32 bytes a lane in two copies fetched every sector twice: 64 us instead of
-// 45 for the 144256 x 128 fp32 backward).
+// neighbouring 16 bytes (32 bytes a lane in two copies fetched every sector twice: 63 us instead of
+// 42 for the 144256 x 128 fp32 backward).
 #pragma once
 #include <type_traits>
 #include "philox.cuh"
