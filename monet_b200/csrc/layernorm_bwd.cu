@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(K * kE<T> >= 32 ? kMaxThreadsWide : kMaxThread
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int i = row + r * step;
-        s[2 * r] = i < rows ? __ldg(sums_of_rows + 2 * static_cast<size_t>(actual(i))) : 0.f;
-        s[2 * r + 1] = i < rows ? __ldg(sums_of_rows + 2 * static_cast<size_t>(actual(i)) + 1) : 0.f;
+        s[2 * r] = i < rows ? __ldcg(sums_of_rows + 2 * static_cast<size_t>(actual(i))) : 0.f;
+        s[2 * r + 1] = i < rows ? __ldcg(sums_of_rows + 2 * static_cast<size_t>(actual(i)) + 1) : 0.f;
       }
     }
     if constexpr (PASS != kStats) {

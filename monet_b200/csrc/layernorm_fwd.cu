@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES)) ln_fwd_rows(LnArgs
 #pragma unroll
       for (int r = 0; r < R; ++r)
         if (first + r * step < rows) {
-          mean_next[r] = __ldg(p.mean + actual(first + r * step));
-          rstd_next[r] = __ldg(p.rstd + actual(first + r * step));
+          mean_next[r] = __ldcg(p.mean + actual(first + r * step));      // written by the kernel before
+          rstd_next[r] = __ldcg(p.rstd + actual(first + r * step));
         }
     }
   };
