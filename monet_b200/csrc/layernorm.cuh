@@ -22,7 +22,6 @@
 #include "rows.cuh"
 
 namespace mb {
-namespace {
 
 struct LnArgs {
   const void *a, *b, *c;       // forward: x, residual; backward: dy, kept, dsum
@@ -35,6 +34,10 @@ struct LnArgs {
   float eps;
   Drop drop;
 };
+// Where the backward's sums over rows go, and its workspace.
+struct Grads { void *dw, *db; float* ws; };
+
+namespace {
 
 // ---- any shape, any stride, any alignment ----------------------------------------------------
 // One CTA per row, element-wise accesses; a row is read again for each of its three uses, from L2
@@ -224,6 +227,27 @@ inline void size_grid(size_t rows, int per_sm, RowPlan* q) {
   q->grid = static_cast<int>(want * unit);
 }
 
+
+inline int column_parts(const mb_ln_desc* d) {
+  const size_t tiles = (d->cols + 31) / 32, groups = (d->rows + 7) / 8;
+  size_t want = (static_cast<size_t>(num_sms()) * 8 + tiles - 1) / tiles;
+  if (want > groups) want = groups;
+  return static_cast<int>(want < 1 ? 1 : want > 1024 ? 1024 : want);
+}
+
+
+// Plan of the row kernel; one CTA per SM, so that there are few partial sums.
+inline bool plan_bwd(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
+  if (!plan_bwd_rows(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, from_y, q)) return false;
+  size_grid(d->rows, 1, q);
+  return true;
+}
+
+inline bool plan_bwd_long(const mb_ln_desc* d, int ops, bool from_y, RowPlan* q) {
+  if (!plan_long(d->rows, d->cols, static_cast<int>(dtype_bytes(d->dtype)), ops, from_y ? 2 : 1, q)) return false;
+  size_grid(d->rows, 1, q);
+  return true;
+}
 
 // The launches of one kernel: its register count (which bounds the CTAs per SM) and the device-side
 // shared-memory limit are looked up once per device.
