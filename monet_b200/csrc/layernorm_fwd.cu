@@ -114,8 +114,11 @@ __global__ void __launch_bounds__(fwd_threads(K, kE<T>, RES)) ln_fwd_rows(LnArgs
   }
   if (!kInRegs) __syncthreads();       // the parameters and the counts
   // Combining the warps' statistics, a lane looks after the warp of its number.  Warps with equal counts,
-  // a power of two of them, merge like lanes.
-  const bool alike = !EDGE && q.chunk == K * q.team && (warps & (warps - 1)) == 0;
+  // a power of two of them, merge like lanes.  The last CTA of a cluster may hold less than its chunk (16-bit
+  // 32760: its last warp is 8 values short) and then merges by its counts.  (Asking the counts themselves gives
+  // the same answer, but not one that the compiler knows to be the whole CTA's: bf16 4096 x 16384 64 us against 61.)
+  const bool full = PASS != kCluster || static_cast<size_t>(at.rank + 1) * q.chunk * E <= p.cols;
+  const bool alike = !EDGE && full && q.chunk == K * q.team && (warps & (warps - 1)) == 0;
   const float part_count = q.team > 32 && lane < warps ? counts[at.group * warps + lane] : 0.f;
   const float part_inv = part_count > 0.f ? 1.f / part_count : 0.f, part_total = q.team > 32 ? warp_sum(part_count) : 0.f;
   const float part_each = part_total > 0.f ? 1.f / part_total : 0.f;
