@@ -141,11 +141,18 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// 1 / v, off by one unit in the last place at most.
+// 1 / v for 2^-126 <= |v| <= 2^126, off by one unit in the last place at most.  (Outside that range v or 1 / v
+// is subnormal, which the instruction takes for zero, or 1 / v overflows.)
 __device__ __forceinline__ float reciprocal(float v) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+__device__ __forceinline__ bool has_reciprocal(float v) { return __float_as_uint(fabsf(v)) - 0x00800000u <= 0x7e000000u; }
+// a / v for any v: at the ends of the range both are moved away from them by a power of two.
+__device__ __forceinline__ float quotient(float a, float v) {
+  const float f = fabsf(v) < 0x1p-60f ? 0x1p64f : fabsf(v) > 0x1p60f ? 0x1p-64f : 1.f;
+  return a * f * reciprocal(v * f);
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
