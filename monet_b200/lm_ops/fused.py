@@ -198,6 +198,7 @@ class OutputActDropoutAddLayerNorm(_DropoutAddLayerNorm):
     """Keeps nothing but the output (which the next operator reads anyway): neither x nor the sum.
     Every weight must be non-zero (ln.OutputActLayerNorm)."""
     backward_storage = [InputStorage(3, 4), OutputStorage()]
+    divides_by = 3
 
     def forward(self, x, residual, normalized_shape, weight=None, bias=None, eps=1e-5, p=0.0, training=True):
         return self._forward(x, residual, normalized_shape, weight, bias, eps, p, training)[0]

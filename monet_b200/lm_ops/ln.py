@@ -48,6 +48,7 @@ class OutputActLayerNorm(_LayerNorm):
     """Backward from the stored OUTPUT y, xhat = (y - bias) / weight: the input is not kept and the
     forward can run in place.  Every weight must be non-zero."""
     backward_storage = [InputStorage(2, 3), OutputStorage()]
+    divides_by = 2                      # position of the argument that must not hold a zero
 
     def backward(self, grad_output, stored, nodel=False):
         with torch.no_grad():

@@ -25,7 +25,7 @@ add -> relu chains into the fused nodes of ``lm_ops/fused.py`` before execution.
 from __future__ import annotations
 
 import operator
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any, Callable, Dict, List, Optional, Tuple
 
 import torch
@@ -293,6 +293,8 @@ def store_all(nodes: List[Node], n: Node) -> Choice:
     return Choice()
 
 
+_LN_LIKE = ('aten::layer_norm', 'monet::dropout_add_layer_norm')
+
 # Producers whose output no backward of their own reads and that return memory of their own: a sole
 # reader may overwrite it.
 _NEVER_READ_AGAIN = ('aten::addmm', 'aten::_convolution', 'aten::add')
@@ -301,10 +303,11 @@ _NEVER_READ_AGAIN = ('aten::addmm', 'aten::_convolution', 'aten::add')
 def low_memory(nodes: List[Node], n: Node) -> Choice:
     """In-place batch norm and layer norm that backpropagate from their output, ReLU kept as nothing at all
     (recomputed from the batch-norm output it reads, gated in backward by that same tensor),
-    residual add in place, max-pool keeping 4-bit indices."""
+    residual add in place, max-pool keeping 4-bit indices.  (A layer norm with a weight of zero keeps its
+    input: ``Runner``.)"""
     if n.op == 'aten::batch_norm':
         return Choice(impl=1, inplace=_sole_user(nodes, n))
-    if n.op in ('aten::layer_norm', 'monet::dropout_add_layer_norm'):
+    if n.op in _LN_LIKE:
         return Choice(impl=1, inplace=_sole_user(nodes, n) and nodes[n.args[0].value].op in _NEVER_READ_AGAIN)
     if n.op == 'monet::dropout':
         return Choice(recompute=True)      # keeps its seed; the same mask is drawn again
@@ -352,7 +355,11 @@ class Runner:
                  fuse: bool = False, channel_sums: bool = True, counter_dropout: bool = False):
         """``fuse`` rewrites the graph (``fuse_graph``); ``counter_dropout`` runs every dropout that
         is not part of a fused node as ``monet::dropout``, which stores no mask and can be
-        recomputed."""
+        recomputed.
+
+        A layer norm that the policy has backpropagate from its output divides by its weight.  Where
+        that holds a zero when the Runner is built (zero-initialised branches), the form that keeps the
+        input takes its place, out of place.  Weights loaded afterwards are not looked at."""
         self.model = model
         self.nodes, self.out_id = extract_graph(model)
         if fuse:
@@ -377,14 +384,24 @@ class Runner:
                     self._param_uses[a.value] = self._param_uses.get(a.value, 0) + 1
         self.shapes: Dict[int, tuple] = {}      # node id -> output shape, filled by forward()
         self._tensors = dict(model.state_dict(keep_vars=True))
+        for n in self.nodes:
+            if self._divides_by_zero(n):
+                self.choices[n.id] = replace(self.choices[n.id], impl=0, inplace=False)
         self._last_fwd_user = {n.id: (max(n.users) if n.users else -1) for n in self.nodes}
         self._validate()
 
     # -- helpers ---------------------------------------------------------------
+    def _impl(self, n: Node):
+        impls = lm_ops.list_ops(self.mode, n.op)
+        return impls[min(self.choices[n.id].impl, len(impls) - 1)]
+
+    def _divides_by_zero(self, n: Node) -> bool:
+        at = getattr(self._impl(n), 'divides_by', None) if n.op in _LN_LIKE else None
+        return at is not None and n.args[at].kind == 'param' and bool((self._tensors[n.args[at].value] == 0).any())
+
     def _new_op(self, n: Node):
         c = self.choices[n.id]
-        impls = lm_ops.list_ops(self.mode, n.op)
-        op = impls[min(c.impl, len(impls) - 1)]()
+        op = self._impl(n)()
         if hasattr(op, 'inplace'):
             op.inplace = c.inplace
         if c.algorithm >= 0:
