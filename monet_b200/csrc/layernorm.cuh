@@ -11,9 +11,10 @@
 //
 // Bound by HBM for large tensors: forward reads and writes each element once, backward reads two or
 // three tensors and writes one or two.  Measured against a copy at 6569 GB/s: forward bf16 16384 x 8192
-// 88 us (0.93), 16384 x 4096 50 us (0.82); backward bf16 16384 x 4096 70 us (0.87), fp32 144256 x 128 from
-// the output 41 us (0.83); with dropout, add and sum bf16 8192 x 2048 forward 32 us (0.64), backward 45 us
-// (0.57), where the generator's instructions and the latency of a row's reductions are what is left.
+// 89 us (0.92), 16384 x 4096 50 us (0.82); backward bf16 16384 x 4096 70 us (0.88), fp32 144256 x 128 from
+// the output 42 us (0.80); with dropout, add and sum bf16 8192 x 2048 forward 32 us (0.64), backward 46 us
+// (0.56), where latency is what is left: the generator stands in series with a row's reductions, and
+// issue is active half of the time.
 // Small calls (a few microseconds) are bound by their launches.
 #pragma once
 #include <atomic>

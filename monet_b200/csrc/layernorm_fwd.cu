@@ -6,12 +6,13 @@ namespace {
 
 // ---- rows in registers -----------------------------------------------------------------------
 // Statistics: every thread centres on its own mean, and (sum, squared deviations) are merged pairwise
-// over the lanes, then over the warps and the CTAs of a cluster: no difference of large sums is ever
-// formed, and one pass over the lanes does.  (Where a warp's lanes hold different numbers of values it
+// over the lanes, then over the warps and the CTAs of a cluster: no large values are squared and
+// subtracted, and one pass over the lanes does.  (Where a warp's lanes hold different numbers of values it
 // centres on the warp's mean instead.)  The chain of shuffles is what a row waits for: bf16 16384 x 4096
 // took 63 us with one pass for the mean and one for the deviations, 57 with the merge.
-// Long rows (PASS): 184 x 200704 fp32 takes 80 us in two passes; held in the shared memory of clusters of
-// eight or sixteen CTAs it took 100, since those leave a fifth of the SMs without work.
+// Long rows (PASS): two passes, 184 x 200704 fp32 91 us on inputs that are not in L2.  Held in the shared memory
+// of clusters of eight or sixteen CTAs it took 100 where two passes took 80, since those leave a fifth of the
+// SMs without work.
 template <int P>
 __device__ __forceinline__ void normalise(float2 (&y)[P], float mean, float rstd, const float2 (&w)[P], const float2 (&b)[P]) {
 #pragma unroll

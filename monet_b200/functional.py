@@ -1043,8 +1043,8 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, inplace: bool = Fa
     """x / (1 - p) where kept, 0 where dropped.  Which elements are dropped depends on `seed` (an
     int64 tensor of one element on x's device, ``dropout_seed``), `offset` (tells dropouts that
     share a seed apart) and the element's position in physical order, so the mask is not stored:
-    ``dropout_bwd`` and a repeated forward draw the same one.  The generator is specified at
-    ``mb_dropout`` in the header."""
+    ``dropout_bwd`` and a repeated forward draw the same one.  `inplace` overwrites a dense x.  The
+    generator is specified at ``mb_dropout`` in the header."""
     code = _act_dtype(x)
     if x.get_device() != _current_device():
         with torch.cuda.device(x.device):
